@@ -1,0 +1,453 @@
+"""Token steps and prompts in low bits, as cases that can be timed and compared: pages handed out on the
+GPU, rows appended to a key / value cache of 8 bits with a scale per page and head, attention off that
+cache, and products with 4-bit weights and group scales.
+
+``run`` is one pass, through the framework's entry points where ``own`` is true and in plain torch
+operations elsewhere; ``exact`` gives the same in 64 bits. Head layouts and matrix sizes are the decoder
+configurations' (32 or 16 query heads over 8 or 4 of keys, 128 or 64 columns), pages the engine's 16
+tokens or a power of two above."""
+from __future__ import annotations
+
+import math
+
+import torch
+
+own = False
+
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+MOST = {"int8": 127.0, "e4m3": 448.0}
+TYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+LEAST = 2.0 ** -100       # the smallest scale of a page
+
+
+def listed():
+    return [
+        # pages for eight live replies' next tokens: latency alone
+        {"name": "pages 8 tokens", "kind": "pages", "seqs": 8, "tokens": 1, "past": 600, "page": 16, "ended": 0, "short": False},
+        # a step of a large server: 500 requests, prompts among them, some ended
+        {"name": "pages 500 requests", "kind": "pages", "seqs": 500, "tokens": 90, "past": 1500, "page": 16, "ended": 23, "short": False},
+        # a token's rows of eight replies into pages that are partly filled
+        {"name": "append 8 tokens", "kind": "append", "seqs": 8, "tokens": 1, "past": 600, "heads": 32, "kv": 8, "dim": 128, "page": 16, "type": "int8", "rope": True},
+        # the rows of a long prompt, and of several odd ones behind cached prefixes
+        {"name": "append prompt 2048", "kind": "append", "seqs": 1, "tokens": 2048, "past": 0, "heads": 32, "kv": 8, "dim": 128, "page": 16, "type": "e4m3", "rope": True},
+        {"name": "append 5 odd prompts", "kind": "append", "seqs": 5, "tokens": 331, "past": 77, "heads": 16, "kv": 4, "dim": 64, "page": 32, "type": "int8", "rope": True},
+        # the attention of a token: one reply, many long ones, one over a very long context
+        {"name": "attend 1 token", "kind": "attend", "seqs": 1, "tokens": 1, "past": 600, "heads": 32, "kv": 8, "dim": 128, "page": 16, "type": "int8"},
+        {"name": "attend 32 tokens", "kind": "attend", "seqs": 32, "tokens": 1, "past": 4000, "heads": 32, "kv": 8, "dim": 128, "page": 16, "type": "int8"},
+        {"name": "attend 1 token of 100000", "kind": "attend", "seqs": 1, "tokens": 1, "past": 100000, "heads": 32, "kv": 8, "dim": 128, "page": 16, "type": "e4m3"},
+        # a prompt's, and chunks of three prompts behind long cached contexts
+        {"name": "attend prompt 2048", "kind": "attend", "seqs": 1, "tokens": 2048, "past": 0, "heads": 32, "kv": 8, "dim": 128, "page": 16, "type": "int8"},
+        {"name": "attend 3 chunks", "kind": "attend", "seqs": 3, "tokens": 113, "past": 5000, "heads": 32, "kv": 8, "dim": 64, "page": 16, "type": "e4m3"},
+        # an attention output projection for one reply, and gate and up of eight
+        {"name": "linear4 1 row", "kind": "linear4", "rows": 1, "n": 4096, "k": 4096, "group": 128, "zeros": False, "bias": False},
+        {"name": "linear4 8 rows", "kind": "linear4", "rows": 8, "n": 28672, "k": 4096, "group": 64, "zeros": True, "bias": False},
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(("pages", "append", "attend", "attend", "linear4"))
+    if kind == "pages":
+        seqs = _log(rng, 1, 700)
+        return {"kind": kind, "seqs": seqs, "tokens": _log(rng, 1, max(1, min(2000, 45000 // seqs))), "past": _log(rng, 1, 3000),
+                "page": rng.choice((16, 16, 32, 64)), "ended": rng.choice((0, 0, seqs // 3)), "short": rng.random() < 0.15}
+    if kind == "linear4":
+        group = rng.choice((32, 64, 128))
+        n, k = 16 * _log(rng, 16, 1792), group * _log(rng, 512 // group, 14336 // group)
+        while n * k > 28672 * 4096:
+            n = 16 * _log(rng, 16, 1792)
+        return {"kind": kind, "rows": _log(rng, 1, 64), "n": n, "k": k, "group": group, "zeros": rng.random() < 0.5, "bias": rng.random() < 0.3}
+    kv = rng.choice((1, 2, 4, 8, 8))
+    case = {"kind": kind, "heads": kv * rng.choice((1, 2, 4, 4, 5, 8)), "kv": kv, "dim": rng.choice((64, 128, 128)),
+            "page": rng.choice((16, 16, 32, 128)), "type": rng.choice(("int8", "e4m3"))}
+    if kind == "append":
+        case["rope"] = rng.random() < 0.8
+    if rng.random() < 0.45:              # token steps, a few tokens each among them
+        case["seqs"], case["tokens"], case["past"] = _log(rng, 1, 64), rng.choice((1, 1, 1, 2, 3)), _log(rng, 1, 6000)
+        if kind == "attend" and rng.random() < 0.25:
+            case["seqs"], case["past"] = rng.choice((1, 2)), _log(rng, 6000, 60000)
+        case["seqs"] = max(1, min(case["seqs"], 128000 * 1024 // (case["past"] * kv * case["dim"])))
+    else:
+        case["seqs"] = rng.choice((1, 1, 2, 3, 7))
+        case["tokens"] = max(1, _log(rng, 16, 2048) // case["seqs"])
+        case["past"] = rng.choice((0, 0, _log(rng, 1, 8000)))
+        most = 2048 * 2048 * 32 * 128 // 2
+        while case["seqs"] * case["tokens"] * (case["past"] + case["tokens"] // 2) * case["heads"] * case["dim"] > most:
+            case["past"], case["tokens"] = case["past"] * 3 // 4, max(1, case["tokens"] * 7 // 8)
+    return case
+
+
+# ------------------------------------------------------------------------------------ inputs
+def _gen(seed, part):
+    return torch.Generator(device="cuda").manual_seed(int(seed) * 7919 + part)
+
+
+def _normal(g, *shape, std=1.0, dtype=BF16):
+    return torch.empty(*shape, dtype=dtype, device="cuda").normal_(0.0, std, generator=g)
+
+
+def _ints(values, dtype=torch.int32):
+    return torch.tensor(values, dtype=dtype, device="cuda")
+
+
+def _lengths(case):
+    """Tokens fed and tokens cached before them, ragged where there are several sequences."""
+    n, t, past = case["seqs"], case["tokens"], case["past"]
+    feeds = [max(1, t - (7 * i) % max(1, t // 2 + 1)) for i in range(n)]
+    return feeds, [max(0, past - 13 * i % max(1, past // 2 + 1)) if past else 0 for i in range(n)]
+
+
+def _tables(g, needs, extra):
+    """A table row per sequence with that many pages each, scattered over a pool; entries behind them 0."""
+    pool = sum(needs) + extra
+    order = torch.randperm(pool, device="cuda", generator=g).to(torch.int32)
+    table, at = torch.zeros(len(needs), max(max(needs), 1), dtype=torch.int32, device="cuda"), 0
+    for i, n in enumerate(needs):
+        table[i, :n] = order[at:at + n]
+        at += n
+    return pool, order, table
+
+
+def _page_scale(top, kind):
+    """The scale of a page whose largest magnitude is ``top``."""
+    s = top / MOST[kind]
+    if kind == "e4m3":                   # the power of two at or above it
+        m, e = torch.frexp(s)
+        s = torch.ldexp(torch.ones_like(s), torch.where(m > 0.5, e, e - 1))
+    return s
+
+
+def _to_bits(x, kind):
+    x = x.clamp(-MOST[kind], MOST[kind])
+    return x.round().to(torch.int8) if kind == "int8" else x.float().to(torch.float8_e4m3fn)
+
+
+def _filled(g, pool, case):
+    """Pages of one of the two caches with rows in them: channels of unlike size, as keys have, and pages of unlike scale."""
+    kv, page, dim, kind = case["kv"], case["page"], case["dim"], case["type"]
+    bits = torch.empty(pool, kv, page, dim, dtype=TYPES[kind], device="cuda")
+    scale = torch.empty(pool, kv, dtype=F32, device="cuda")
+    size = (0.3 + 1.2 * torch.rand(kv, 1, dim, device="cuda", generator=g))
+    for a in range(0, pool, 4096):       # a part of the pool at a time
+        x = _normal(g, min(4096, pool - a), kv, page, dim, dtype=F32) * size
+        s = _page_scale(x.abs().amax((2, 3)), kind).clamp_min(LEAST)
+        bits[a:a + 4096], scale[a:a + 4096] = _to_bits(x / s[..., None, None], kind), s
+    return bits, scale
+
+
+def _cos_sin(dim, rows):
+    inv = 1.0 / (500000.0 ** (torch.arange(0, dim, 2, dtype=F64) / dim))
+    ang = torch.arange(rows, dtype=F64)[:, None] * inv[None, :]
+    return torch.stack([ang.cos(), ang.sin()], -1).to(F32).cuda()
+
+
+def _inputs(case, seed):
+    kind = case["kind"]
+    if kind == "pages":
+        g, page = _gen(seed, 1), case["page"]
+        feeds, pasts = _lengths(case)
+        ended = set(range(0, 3 * case["ended"], 3))
+        feeds = [-1 if i in ended else n for i, n in enumerate(feeds)]
+        held = [-(-c // page) for c in pasts]
+        wanted = sum(-(-(c + max(n, 0)) // page) - h for c, n, h in zip(pasts, feeds, held))
+        free = wanted + 9 if not case["short"] else max(0, wanted - 1)
+        pool, order, table = _tables(g, held, free)
+        table = torch.nn.functional.pad(table, (0, -(-max(0, max(feeds)) // page) + 2))
+        head = (int(seed) * 31 + 5) % pool
+        ring = torch.zeros(pool, dtype=torch.int32, device="cuda")
+        ring[(torch.arange(free, device="cuda") + head) % pool] = order[pool - free:]
+        total = sum(max(n, 0) for n in feeds)
+        return {"new": _ints(feeds), "ctx": _ints(pasts), "table": table, "free": ring, "ring": _ints([head, free]),
+                "most": -(-total // 8) * 8 + 8}
+    if kind == "linear4":
+        g, n, k, group = _gen(seed, 2), case["n"], case["k"], case["group"]
+        return {"x": _normal(g, case["rows"], k), "bits": torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=g),
+                "scales": (0.004 * (0.5 + torch.rand(n, k // group, device="cuda", generator=g))).to(BF16),
+                "zeros": torch.randint(4, 12, (n, k // group), dtype=torch.uint8, device="cuda", generator=g) if case["zeros"] else None,
+                "bias": _normal(g, n) if case["bias"] else None}
+    g, heads, kv, dim, page = _gen(seed, 3), case["heads"], case["kv"], case["dim"], case["page"]
+    feeds, pasts = _lengths(case)
+    ctx = [n + c for n, c in zip(feeds, pasts)]
+    pool, _, table = _tables(g, [-(-c // page) for c in ctx], 7)
+    s = {"feeds": feeds, "pasts": pasts, "table": table, "ctx": _ints(ctx), "cu": _ints([sum(feeds[:i]) for i in range(len(feeds) + 1)])}
+    s["k"], s["ks"] = _filled(g, pool, case)
+    s["v"], s["vs"] = _filled(g, pool, case)
+    if kind == "append":
+        # rows larger than the cached ones now and then, so that pages' scales have to grow
+        s["qkv"] = _normal(g, sum(feeds), (heads + 2 * kv) * dim) * (1.0 + 2.0 * (torch.rand(sum(feeds), 1, device="cuda", generator=g) < 0.2)).to(BF16)
+        s["cos_sin"] = _cos_sin(dim, max(ctx)) if case["rope"] else None
+        first = [c // page * page for c in pasts]
+        rows = [c - f for c, f in zip(ctx, first)]
+        s["first"], s["cu_read"] = _ints(first), _ints([sum(rows[:i]) for i in range(len(rows) + 1)])
+        s["rows"] = rows
+    else:
+        s["q"] = _normal(g, sum(feeds), heads * dim, std=1.5)
+    return s
+
+
+def prepare(case, seed):
+    s = dict(_inputs(case, seed), case=case)
+    if own:
+        from loqa_hub_amd.ops import lowbit
+        if case["kind"] == "linear4":
+            s["w"] = lowbit.Weight4(s["bits"], s["scales"], s["zeros"])
+        elif case["kind"] != "pages":
+            s["cache"] = lowbit.Cache8(s["k"], s["v"], s["ks"], s["vs"])
+    return s
+
+
+# ------------------------------------------------------------------------------------ one pass
+def run(s):
+    case = s["case"]
+    kind = case["kind"]
+    if not own:
+        return {"pages": _pages, "append": _append, "attend": _attend, "linear4": _linear4}[kind](s, case)
+    from loqa_hub_amd.ops import lowbit
+    if kind == "pages":
+        r = lowbit.page_step(s["new"], s["ctx"], s["table"], s["free"], s["ring"], block_size=case["page"], max_tokens=s["most"])
+        return {"cu_q": r.cu_q, "positions": r.positions, "slots": r.slots, "last_rows": r.last_rows, "ctx_lens": r.ctx_lens,
+                "ring": r.ring, "status": r.status, "table": s["table"], "free": s["free"]}
+    if kind == "linear4":
+        return lowbit.linear4(s["x"], s["w"], s["bias"])
+    if kind == "append":
+        q = lowbit.rope_append8(s["qkv"], s["cos_sin"], s["cache"], s["cu"], s["ctx"], s["table"], n_heads=case["heads"], max_q=max(s["feeds"]))
+        k, v = lowbit.read8(s["cache"], s["cu_read"], s["first"], s["table"], total=sum(s["rows"]))
+        return {"q": q, "k": k, "v": v}
+    return lowbit.attention8(s["q"], s["cache"], s["cu"], s["ctx"], s["table"], n_heads=case["heads"], max_q=max(s["feeds"]),
+                             max_k=max(a + b for a, b in zip(s["feeds"], s["pasts"])))
+
+
+def _pages(s, case):
+    page, pool, (B, width) = case["page"], s["free"].numel(), s["table"].shape
+    dev, i64 = s["free"].device, torch.int64
+    new, ctx, head, count = s["new"].to(i64), s["ctx"].to(i64), s["ring"][0].to(i64), s["ring"][1].to(i64)
+    fed, ended = new.clamp_min(0), new == -1
+    held, after = (ctx + page - 1) // page, torch.where(ended, 0, ctx + fed)
+    want = (ctx + fed + page - 1) // page - held
+    back = torch.where(ended, held, 0)
+    status = torch.where(want.sum() > count, 1, 0) + torch.where(fed.sum() > s["most"], 2, 0) + torch.where((ctx + fed > width * page).any(), 4, 0)
+    ok = status == 0
+    ends, first, given = torch.cumsum(fed, 0), torch.cumsum(want, 0) - want, torch.cumsum(back, 0) - back
+    # a place (row, column) of the table: held before, handed out now, or given back
+    col = torch.arange(width, device=dev)
+    gone = ended[:, None] & (col < held[:, None]) & ok
+    at = torch.where(gone, (head + count + given[:, None] + col) % pool, pool)
+    free = torch.cat([s["free"], s["free"].new_zeros(1)]).scatter(0, at.reshape(-1), s["table"].reshape(-1))[:pool]
+    fresh = (col >= held[:, None]) & (col < (held + want)[:, None]) & ok
+    table = torch.where(fresh, s["free"][((head + first[:, None] + col - held[:, None]) % pool)], s["table"])
+    s["table"].copy_(table)
+    s["free"].copy_(free)
+    t = torch.arange(s["most"], device=dev)
+    b = torch.searchsorted(ends, t, right=True).clamp_max(B - 1)
+    live = (t < ends[-1]) & ok
+    pos = torch.where(live, (ctx + fed - ends)[b] + t, 0)
+    slots = torch.where(live, table[b, (pos // page).clamp_max(width - 1)].to(i64) * page + pos % page, -1)
+    i32 = torch.int32
+    return {"cu_q": torch.where(ok, torch.nn.functional.pad(ends, (1, 0)), 0).to(i32), "positions": pos.to(i32), "slots": slots.to(i32),
+            "last_rows": torch.where(ok & (fed > 0), ends - 1, 0), "ctx_lens": torch.where(ok, after, ctx).to(i32),
+            "ring": torch.where(ok, torch.stack([(head + want.sum()) % pool, count - want.sum() + back.sum()]), s["ring"]).to(i32),
+            "status": status.to(i32).reshape(1), "table": s["table"], "free": s["free"]}
+
+
+def _rotated(x, cs):
+    """x [T, heads, D] in f32 turned by the table's rows: halves a, b -> a c - b s, b c + a s."""
+    a, b = x.chunk(2, -1)
+    c, s = cs[:, None, :, 0], cs[:, None, :, 1]
+    return torch.cat([a * c - b * s, b * c + a * s], -1)
+
+
+def _append(s, case):
+    H, G, D, page, kind = case["heads"], case["kv"], case["dim"], case["page"], case["type"]
+    T, B, i64 = s["qkv"].shape[0], len(s["feeds"]), torch.int64
+    x = s["qkv"].float().view(T, H + 2 * G, D)
+    qk, v = x[:, :H + G], x[:, H + G:]
+    cu, ctx = s["cu"].to(i64), s["ctx"].to(i64)
+    b = torch.searchsorted(cu[1:], torch.arange(T, device=cu.device), right=True)
+    pos = (ctx - cu[1:])[b] + torch.arange(T, device=cu.device)
+    if s["cos_sin"] is not None:
+        qk = _rotated(qk, s["cos_sin"][pos])
+    # the pages that get rows, one after the other, and each row's among them
+    lo, hi = [c // page for c in s["pasts"]], [-(-(c + n) // page) for c, n in zip(s["pasts"], s["feeds"])]
+    pages = torch.cat([s["table"][i, lo[i]:hi[i]] for i in range(B)]).to(i64)
+    start = (ctx - cu[1:] + cu[:-1]) // page
+    each = (ctx + page - 1) // page - start
+    place = ((torch.cumsum(each, 0) - each) - start)[b] + pos // page
+    for bits, scale, rows in ((s["k"], s["ks"], qk[:, H:]), (s["v"], s["vs"], v)):
+        n = pages.numel()
+        top = torch.zeros(n, G, device=cu.device).scatter_reduce(0, place[:, None].expand(-1, G), rows.abs().amax(-1), "amax")
+        anew = torch.zeros(n, dtype=torch.int32, device=cu.device).scatter_reduce(0, place, (pos % page == 0).int(), "amax") > 0
+        had = scale[pages]
+        now = torch.maximum(torch.where(anew[:, None], 0.0, had), _page_scale(top, kind)).clamp_min(LEAST)
+        old = bits[pages].float() * had[..., None, None]
+        keep = (now == had)[..., None, None]
+        kept = torch.where(keep, bits[pages].float(), _to_bits(old / now[..., None, None], kind).float()).to(bits.dtype)
+        kept[place, :, pos % page] = _to_bits(rows / now[place][..., None], kind)
+        bits[pages], scale[pages] = kept, now
+    k, v = (_read(s[a], s[a + "s"], s, page) for a in "kv")
+    return {"q": qk[:, :H].reshape(T, H * D).to(BF16), "k": k, "v": v}
+
+
+def _read(bits, scale, s, page):
+    """The rows of the touched pages as what they stand for."""
+    out = []
+    for i, n in enumerate(s["rows"]):
+        lo = s["pasts"][i] // page
+        at = s["table"][i, lo:lo + -(-n // page)].to(torch.int64)
+        out.append((bits[at].float() * scale[at][..., None, None]).transpose(1, 2).flatten(0, 1)[:n])
+    return torch.cat(out).to(BF16)
+
+
+def _attend(s, case):
+    H, G, D, page = case["heads"], case["kv"], case["dim"], case["page"]
+    out, at = [], 0
+    for i, (n, past) in enumerate(zip(s["feeds"], s["pasts"])):
+        L = n + past
+        pages = s["table"][i, :-(-L // page)].to(torch.int64)
+        k, v = ((bits[pages].float() * scale[pages][..., None, None]).transpose(0, 1).flatten(1, 2)[:, :L]
+                for bits, scale in ((s["k"], s["ks"]), (s["v"], s["vs"])))
+        q = s["q"][at:at + n].float().view(n, G, H // G, D).permute(1, 2, 0, 3).reshape(G, -1, D)
+        w = torch.matmul(q, k.transpose(1, 2)) * (1.0 / math.sqrt(D))
+        if n > 1:
+            hide = torch.arange(L, device=w.device)[None] > past + torch.arange(n, device=w.device)[:, None]
+            w = w.view(G, H // G, n, L).masked_fill(hide, -math.inf).view(G, -1, L)
+        w = torch.exp(w - w.amax(-1, keepdim=True))
+        o = torch.matmul(w, v) / w.sum(-1, keepdim=True)
+        out.append(o.view(G, H // G, n, D).permute(2, 0, 1, 3).reshape(n, H * D))
+        at += n
+    return torch.cat(out).to(BF16)
+
+
+def _linear4(s, case):
+    n, k, group = case["n"], case["k"], case["group"]
+    bits = torch.stack([s["bits"] & 15, s["bits"] >> 4], -1).view(n, k // group, group).float()
+    zero = 8.0 if s["zeros"] is None else s["zeros"].float()[..., None]
+    w = ((bits - zero) * s["scales"].float()[..., None]).view(n, k)
+    y = torch.matmul(s["x"].float(), w.t())
+    if s["bias"] is not None:
+        y = y + s["bias"].float()
+    return y.to(BF16)
+
+
+# ------------------------------------------------------------------------------------ what a pass cannot do without
+def work(case):
+    kind = case["kind"]
+    feeds, pasts = _lengths(case) if "seqs" in case else ([], [])
+    if kind == "pages":
+        page = case["page"]
+        pages = sum(-(-(c + n) // page) - c // page for c, n in zip(pasts, feeds))
+        return {"bytes": 32 * len(feeds) + 8 * sum(feeds) + 8 * pages, "flops": 4 * len(feeds) + 4 * sum(feeds)}
+    if kind == "linear4":
+        n, k, m, per = case["n"], case["k"], case["rows"], 2 + (1 if case["zeros"] else 0)
+        return {"bytes": n * k // 2 + n * k // case["group"] * per + 2 * m * (n + k) + (2 * n if case["bias"] else 0), "flops": 2 * m * n * k}
+    H, G, D, page = case["heads"], case["kv"], case["dim"], case["page"]
+    T = sum(feeds)
+    if kind == "append":
+        cached = sum(c % page for c in pasts)                # rows of pages that get new ones
+        return {"bytes": T * (2 * (H + 2 * G) * D + 2 * H * D + 2 * G * D) + (4 * T * D if case["rope"] else 0)
+                + 2 * G * D * 3 * (T + cached),              # the touched rows read back: a byte in, two out
+                "flops": 6 * T * (H + G) * D + 6 * T * G * D}
+    seen = sum(n * c + n * (n + 1) // 2 for n, c in zip(feeds, pasts))
+    keys = sum(n + c for n, c in zip(feeds, pasts))
+    return {"bytes": 2 * keys * G * D + 8 * G * (keys // page + 1) + 4 * T * H * D, "flops": 4 * seen * H * D}
+
+
+# ------------------------------------------------------------------------------------ in 64 bits
+def exact(case, seed):
+    s, kind = _inputs(case, seed), case["kind"]
+    if kind == "pages":
+        return _exact_pages(s, case)
+    if kind == "linear4":
+        y = torch.empty(case["rows"], case["n"], dtype=F64, device="cuda")
+        x, per = s["x"].to(F64), case["group"]
+        for a in range(0, case["n"], 1024):                  # some features at a time
+            nib = s["bits"][a:a + 1024].to(torch.int64)
+            w = torch.empty(nib.shape[0], case["k"], dtype=F64, device="cuda")
+            w[:, 0::2], w[:, 1::2] = (nib % 16).to(F64), (nib // 16).to(F64)
+            w -= 8 if s["zeros"] is None else s["zeros"][a:a + 1024].to(F64).repeat_interleave(per, 1)
+            w *= s["scales"][a:a + 1024].to(F64).repeat_interleave(per, 1)
+            y[:, a:a + 1024] = x @ w.t().contiguous()
+        return y if s["bias"] is None else y + s["bias"].to(F64)
+    H, G, D, page = case["heads"], case["kv"], case["dim"], case["page"]
+    if kind == "attend":
+        out, at = torch.empty(s["q"].shape, dtype=F64, device="cuda"), 0
+        for i, (n, past) in enumerate(zip(s["feeds"], s["pasts"])):
+            L = n + past
+            rows = torch.arange(L, device="cuda")
+            where, inside = s["table"][i].long()[rows // page], rows % page
+            for g in range(G):
+                k = s["k"][where, g, inside].to(F64) * s["ks"][where, g].to(F64)[:, None]
+                v = s["v"][where, g, inside].to(F64) * s["vs"][where, g].to(F64)[:, None]
+                for h in range(g * (H // G), (g + 1) * (H // G)):
+                    w = s["q"][at:at + n, h * D:(h + 1) * D].to(F64) @ k.t().contiguous() / D ** 0.5
+                    w = w.masked_fill(rows[None] > past + torch.arange(n, device="cuda")[:, None], -math.inf)
+                    out[at:at + n, h * D:(h + 1) * D] = torch.softmax(w, -1) @ v
+            at += n
+        return out
+    # append: a sequence at a time, its rows and what is left of its first page
+    qkv, half = s["qkv"].to(F64).view(-1, H + 2 * G, D), D // 2
+    keys, values, at = [], [], 0
+    q = torch.empty(qkv.shape[0], H, D, dtype=F64, device="cuda")
+    for i, (n, past) in enumerate(zip(s["feeds"], s["pasts"])):
+        x = qkv[at:at + n].clone()
+        if s["cos_sin"] is not None:
+            c, sn = s["cos_sin"][past:past + n].to(F64).unbind(-1)
+            a, b = x[:, :H + G, :half].clone(), x[:, :H + G, half:].clone()
+            x[:, :H + G, :half] = a * c[:, None] - b * sn[:, None]
+            x[:, :H + G, half:] = b * c[:, None] + a * sn[:, None]
+        q[at:at + n] = x[:, :H]
+        lo = past // page * page
+        for bits, scale, new, out in ((s["k"], s["ks"], x[:, H:H + G], keys), (s["v"], s["vs"], x[:, H + G:], values)):
+            for p in range(lo, past + n, page):
+                id_ = s["table"][i, p // page].long()
+                first, last = max(past, p), min(past + n, p + page)
+                rows = new[first - past:last - past]
+                had = scale[id_].to(F64)
+                need = rows.abs().amax((0, 2)) / MOST[case["type"]]
+                if case["type"] == "e4m3":
+                    need = torch.exp2(torch.ceil(torch.log2(need)))
+                now = torch.maximum(need, had) if first > p else need
+                body = torch.cat([bits[id_, :, :first - p].to(F64).transpose(0, 1) * had[None, :, None], rows]) / now[None, :, None]
+                if case["type"] == "int8":
+                    body = body.round()
+                else:
+                    # a value's step: 2^-3 of its power of two, 2^-9 at the least
+                    step = torch.exp2(torch.floor(torch.log2(body.abs().clamp_min(2.0 ** -6))) - 3)
+                    body = ((body / step).round() * step).clamp(-448, 448)
+                out.append(body * now[None, :, None])
+        at += n
+    return {"q": q.view(-1, H * D), "k": torch.cat(keys), "v": torch.cat(values)}
+
+
+def _exact_pages(s, case):
+    page, table, free = case["page"], s["table"].tolist(), s["free"].tolist()
+    new, ctx, (head, count), pool = s["new"].tolist(), s["ctx"].tolist(), s["ring"].tolist(), s["free"].numel()
+    want = [-(-(c + max(n, 0)) // page) - -(-c // page) for n, c in zip(new, ctx)]
+    total = sum(max(n, 0) for n in new)
+    status = (1 if sum(want) > count else 0) + (2 if total > s["most"] else 0) + (4 if any(c + n > len(table[0]) * page for n, c in zip(new, ctx)) else 0)
+    pos, slots, cu, last, after = [], [], [0], [], []
+    if status == 0:
+        tail = (head + count) % pool
+        for n, c, row in zip(new, ctx, table):
+            held = -(-c // page)
+            if n < 0:
+                for p in row[:held]:
+                    free[tail] = p
+                    tail, count = (tail + 1) % pool, count + 1
+                n = c = 0
+            for j in range(held, -(-(c + n) // page)):
+                row[j] = free[head]
+                head, count = (head + 1) % pool, count - 1
+            pos += range(c, c + n)
+            slots += [row[p // page] * page + p % page for p in range(c, c + n)]
+            cu.append(cu[-1] + n)
+            last.append(cu[-1] - 1 if n else 0)
+            after.append(c + n)
+    else:
+        cu, last, after = [0] * (len(new) + 1), [0] * len(new), ctx
+    rest = s["most"] - len(pos)
+    i64 = torch.int64
+    return {"cu_q": _ints(cu, i64), "positions": _ints(pos + [0] * rest, i64), "slots": _ints(slots + [-1] * rest, i64), "last_rows": _ints(last, i64),
+            "ctx_lens": _ints(after, i64), "ring": _ints([head, count], i64), "status": _ints([status], i64), "table": _ints(table, i64), "free": _ints(free, i64)}
