@@ -116,7 +116,7 @@ def _page_scale(top, kind):
     s = top / MOST[kind]
     if kind == "e4m3":                   # the power of two at or above it
         m, e = torch.frexp(s)
-        s = torch.ldexp(torch.ones_like(s), torch.where(m > 0.5, e, e - 1))
+        s = torch.where(s > 0, torch.ldexp(torch.ones_like(s), torch.where(m > 0.5, e, e - 1)), s)
     return s
 
 
