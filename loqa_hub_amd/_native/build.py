@@ -1,17 +1,18 @@
 """Build the native HIP/C++ libraries in-tree for gfx950.
 
-Four shared objects are produced next to this file:
+Five shared objects are produced next to this file:
 
 * ``libloqa_kernels.so`` - every hand-written CDNA4 kernel under ``csrc/kernels``
-  (compiled with ``hipcc --offload-arch=gfx950``) but the sequence mixers'.
+  (compiled with ``hipcc --offload-arch=gfx950``) but those of the next two.
 * ``libloqa_seqmix.so`` - the sequence-mixer kernels.
+* ``libloqa_lowbit.so`` - the 8-bit cache's and 4-bit weights' kernels.
 * ``libloqa_runtime.so`` - the host runtime under ``csrc/runtime`` (pinned PCM
   staging, paged-KV block pool).
 * ``libloqa_launch.so`` - a Python module, ``csrc/launch``: entry points of token
   steps that take tensors as they are.
 
-The first three are loaded with ctypes *after* ``import torch`` so the process shares
-torch's single HIP runtime (both link ``libamdhip64.so.7``).
+All but the last are loaded with ctypes *after* ``import torch`` so the process shares
+torch's single HIP runtime (all link ``libamdhip64.so.7``).
 
 Usage: ``python -m loqa_hub_amd._native.build [--force] [--debug]``.
 """
@@ -96,6 +97,8 @@ SEQMIX_SOURCES = ("norm_dyt.hip", "attn_latent.hip", "attn_latent_prefill.hip", 
                   "delta_chunks.hip", "moe_pipe.hip", "attn_window_pipe.hip", "attn_window_token.hip",
                   "latent_kv.hip", "head_product.hip")
 
+LOWBIT_SOURCES = ("cache8.hip", "attn_cache8.hip", "linear4.hip")
+
 # hipcc may not form packed-f32 VALU instructions from scalar float code
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
@@ -139,15 +142,18 @@ def build(force: bool = False, debug: bool = False, only=None, quiet: bool = Fal
               f"-I{os.path.join(CSRC, 'kernels')}", *NO_PACKED_F32]
     allk = sorted(glob.glob(os.path.join(CSRC, "kernels", "*.hip")))
     ssrc = [p for p in allk if os.path.basename(p) in SEQMIX_SOURCES]
-    ksrc = [p for p in allk if os.path.basename(p) not in SEQMIX_SOURCES]
+    lsrc = [p for p in allk if os.path.basename(p) in LOWBIT_SOURCES]
+    ksrc = [p for p in allk if os.path.basename(p) not in SEQMIX_SOURCES + LOWBIT_SOURCES]
     allh = sorted(glob.glob(os.path.join(CSRC, "kernels", "*.h")))
-    khdr = [p for p in allh if os.path.basename(p) != "seqmix.h"]
+    khdr = [p for p in allh if os.path.basename(p) not in ("seqmix.h", "cache8.h")]
+    lhdr = [p for p in allh if os.path.basename(p) in ("common.h", "cache8.h", "flash_pipe.h")]
     shdr = [p for p in allh if os.path.basename(p) in ("common.h", "seqmix.h", "gemm_pipe.h", "flash_pipe.h")]
     rsrc = sorted(glob.glob(os.path.join(CSRC, "runtime", "*.cpp")))
     rhdr = sorted(glob.glob(os.path.join(CSRC, "runtime", "*.h")))
     rflags = [*opt, "-std=c++17", "-D__HIP_PLATFORM_AMD__"]
     libs = [("libloqa_kernels.so", ksrc, khdr, kflags),
             ("libloqa_seqmix.so", ssrc, shdr, kflags),
+            ("libloqa_lowbit.so", lsrc, lhdr, kflags),
             ("libloqa_runtime.so", rsrc, rhdr, rflags)]
     out = []
     for name, src, hdr, flags in libs:

@@ -293,6 +293,17 @@ _SEQMIX_SIGS = {
 }
 _seqmix = None
 
+_LOWBIT_SIGS = {
+    "loqa_rope_append8": [_vp, _l, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
+    "loqa_read8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
+    "loqa_attention8": [_vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _vp, _l, _vp, _l,
+                        _vp],
+    "loqa_page_step": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
+    "loqa_shuffle4": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
+    "loqa_linear4": [_vp, _l, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _vp],
+}
+_lowbit = None
+
 
 class NativeLibraryMissing(RuntimeError):
     pass
@@ -310,7 +321,7 @@ _dispatch = None
 
 
 def kernels():
-    """The kernel entry points (both kernel libraries, each loaded on first use)."""
+    """The kernel entry points (the kernel libraries, each loaded on first use)."""
     global _dispatch
     if _dispatch is None:
         _dispatch = _Kernels()
@@ -366,12 +377,14 @@ def launch():
 
 class _Kernels:
     """Attribute lookup over the kernel libraries: the sequence-mixer entry
-    points live in ``libloqa_seqmix.so``, everything else in
+    points live in ``libloqa_seqmix.so``, those of low bits in ``libloqa_lowbit.so``, everything else in
     ``libloqa_kernels.so`` (loaded only when one of its kernels is called)."""
 
     def __getattr__(self, name: str):
         if name in _LAUNCH:
             fn = getattr(launch(), name)
+        elif name in _LOWBIT_SIGS:
+            fn = getattr(lowbit(), name)
         elif name in _SEQMIX_SIGS or name == "loqa_delta_chunks_ws":
             fn = getattr(seqmix(), name)
         else:
@@ -396,6 +409,20 @@ def seqmix() -> ctypes.CDLL:
     return _seqmix
 
 
+def lowbit() -> ctypes.CDLL:
+    global _lowbit
+    if _lowbit is None:
+        with _lock:
+            if _lowbit is None:
+                lib = _load("libloqa_lowbit.so")
+                for fn, sig in _LOWBIT_SIGS.items():
+                    f = getattr(lib, fn)
+                    f.argtypes = sig
+                    f.restype = c_int
+                _lowbit = lib
+    return _lowbit
+
+
 def runtime() -> ctypes.CDLL:
     global _runtime
     if _runtime is None:
@@ -414,6 +441,7 @@ def load_all() -> None:
     """Load every native library (a missing one raises)."""
     _main_kernels()
     seqmix()
+    lowbit()
     launch()
     runtime()
 

@@ -1,0 +1,371 @@
+"""Ops of a serving step in low bits: a paged key / value cache of 8 bits with a scale for each page and
+kv head, the rotation and append that write it, attention off it for tokens and prompts, the pages and
+slots of a step handed out on the GPU, and products with 4-bit weights and group scales.
+
+They stand beside their bf16 counterparts in ``ops`` (:func:`ops.rope_kv_append`, :func:`ops.attention`,
+:func:`ops.linear`) and the engine's host block pool. A step of one token is bound by the bytes of weights
+and cache that it reads: half of them here for the cache, a quarter for the weights.
+
+As everywhere in ``ops``: GPU tensors run the HIP kernels (``csrc/kernels/cache8.hip``,
+``attn_cache8.hip``, ``linear4.hip``), CPU tensors the PyTorch references. Rows are bfloat16; scales,
+softmax and sums are f32.
+
+Sequences are given as everywhere: ``cu_q`` [B + 1] int32 bounds each sequence's rows, ``ctx_lens`` [B]
+int32 its tokens with this step's, ``block_tables`` [B, max_blocks] int32 its pages; row i of a sequence
+of n rows stands at position ctx - n + i. Rows behind the last sequence are neither read nor written.
+Page numbers outside of the cache are never followed: nothing is appended there, and attention takes its
+keys as masked. A page that gets rows belongs to one sequence; full pages may be shared.
+"""
+from __future__ import annotations
+
+import contextlib
+import math
+from typing import NamedTuple
+
+import torch
+
+from . import reference as ref
+from . import _sk_workspace
+from ._lib import check, kernels, ptr, stream_ptr
+
+CACHE_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+HEAD_DIMS = (64, 128)
+TOKEN_ROWS, PROMPT_ROWS = 16, 128     # rows of a workgroup of the two forms (csrc/kernels/attn_cache8.hip)
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _typed(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+
+
+def _i32(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+    _typed(t, torch.int32, name)
+    _need(t.is_contiguous(), f"{name} must be contiguous")
+    _need(t.device == like.device, f"{name} must be on {like.device}")
+
+
+def _device(t: torch.Tensor):
+    """Launches go to the tensors' own device, whichever is the current one."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+class Cache8:
+    """A layer's paged cache in 8 bits: ``k``, ``v`` [n_blocks, n_kv, block_size, head_dim] int8 or
+    float8_e4m3fn codes and ``k_scale``, ``v_scale`` [n_blocks, n_kv] f32: an entry stands for code * scale.
+    A page's scale starts anew with the row at its first place and only grows until the next such row; its
+    older rows are rounded again where it grows, so a page filled row by row is off by up to a step where one filled at
+    once is off by half a step. e4m3 scales are powers of two, whose growth rounds nothing again but the smallest
+    entries. Scales below 2^-100 count as 2^-100. Page sizes are powers of two from 16 on."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "kind", "n_blocks", "n_kv", "block_size", "head_dim")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        if k.dtype not in CACHE_TYPES:
+            raise TypeError(f"a cache of int8 or float8_e4m3fn, got {k.dtype}")
+        _typed(v, k.dtype, "v")
+        _typed(k_scale, torch.float32, "k_scale")
+        _typed(v_scale, torch.float32, "v_scale")
+        _need(k.dim() == 4 and v.shape == k.shape, "k and v are [n_blocks, n_kv, block_size, head_dim]")
+        _need(k_scale.shape == k.shape[:2] and v_scale.shape == k.shape[:2], "scales are [n_blocks, n_kv]")
+        _need(all(t.is_contiguous() and t.device == k.device for t in (k, v, k_scale, v_scale)), "contiguous tensors of one device")
+        _need((k.data_ptr() | v.data_ptr()) % 16 == 0, "k and v must start at 16 bytes")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.kind = CACHE_TYPES[k.dtype]
+        self.n_blocks, self.n_kv, self.block_size, self.head_dim = k.shape
+        _need(self.n_blocks > 0 and self.n_kv > 0, "a cache without pages")
+        _need(self.head_dim in HEAD_DIMS, f"head_dim is one of {HEAD_DIMS}, got {self.head_dim}")
+        _need(self.block_size >= 16 and self.block_size & (self.block_size - 1) == 0, "block_size is a power of two from 16 on")
+        _need(self.n_blocks * self.block_size < 1 << 31, "slots of 32 bits")
+
+    @classmethod
+    def empty(cls, n_blocks: int, n_kv: int, block_size: int, head_dim: int, dtype=torch.int8, device=None) -> "Cache8":
+        if dtype not in CACHE_TYPES:
+            raise TypeError(f"a cache of int8 or float8_e4m3fn, got {dtype}")
+        shape = (n_blocks, n_kv, block_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for _ in range(2))
+        return cls(k, v, torch.zeros(shape[:2], device=device), torch.zeros(shape[:2], device=device))
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
+
+    @staticmethod
+    def bytes_per_block(n_kv: int, head_dim: int, block_size: int) -> int:
+        return 2 * n_kv * (block_size * head_dim + 4)
+
+
+def _sequences(cu_q, ctx_lens, block_tables, like) -> tuple[int, int]:
+    for t, name in ((cu_q, "cu_q"), (ctx_lens, "ctx_lens"), (block_tables, "block_tables")):
+        _i32(t, name, like)
+    B = ctx_lens.numel()
+    _need(cu_q.numel() == B + 1 and block_tables.dim() == 2 and block_tables.shape[0] == B, "cu_q [B + 1], ctx_lens [B], block_tables [B, max_blocks]")
+    _need(B == 0 or block_tables.shape[1] > 0, "a block table without columns")
+    return B, block_tables.shape[1]
+
+
+def _rows(t: torch.Tensor, cols: int, name: str, like) -> None:
+    _typed(t, torch.bfloat16, name)
+    _need(t.dim() == 2 and t.shape[1] >= cols and (t.stride(1) == 1 or t.shape[1] == 1), f"{name} must be rows of at least {cols} columns")
+    _need(t.shape[0] <= 1 or t.stride(0) >= cols, f"rows of {name} must not overlap")
+    _need(t.device == like.device, f"{name} must be on {like.device}")
+
+
+def rope_append8(qkv: torch.Tensor, cos_sin: torch.Tensor | None, cache: Cache8, cu_q: torch.Tensor, ctx_lens: torch.Tensor,
+                 block_tables: torch.Tensor, *, n_heads: int, max_q: int, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotate q and k of a step and append k / v to the cache; returns the rotated queries [T, H * D] bf16 (``q_out``
+    where given).
+
+    qkv: [T, >= (H + 2 Hkv) * D] bf16, q | k | v; cos_sin: [max_pos, D/2, 2] f32 or None (no rotation), which covers every
+    position (rows past its end are turned by its last entry). ``max_q`` bounds the rows of a sequence. Rotated keys
+    go to their codes without a rounding in between. Rows at positions below zero or past the block table are not
+    appended. An infinite or NaN entry makes its page's scale so, and with it what attention gives for the page."""
+    H, G, D = n_heads, cache.n_kv, cache.head_dim
+    _need(H > 0 and max_q >= 0, "n_heads and max_q")
+    _rows(qkv, (H + 2 * G) * D, "qkv", cache)
+    T = qkv.shape[0]
+    B, max_blocks = _sequences(cu_q, ctx_lens, block_tables, cache)
+    if cos_sin is not None:
+        _typed(cos_sin, torch.float32, "cos_sin")
+        _need(cos_sin.dim() == 3 and cos_sin.shape[1:] == (D // 2, 2) and cos_sin.shape[0] > 0 and cos_sin.is_contiguous()
+              and cos_sin.device == cache.device and cos_sin.data_ptr() % 16 == 0, "cos_sin is [max_pos, head_dim / 2, 2], contiguous")
+    if q_out is None:
+        q_out = torch.empty(T, H * D, dtype=torch.bfloat16, device=qkv.device)
+    else:
+        _rows(q_out, H * D, "q_out", cache)
+        _need(q_out.shape[0] == T, "q_out has the rows of qkv")
+    if T == 0 or B == 0 or max_q == 0:
+        return q_out
+    if not qkv.is_cuda:
+        return ref.rope_append8(qkv, cos_sin, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, q_out=q_out)
+    _need((qkv.data_ptr() | q_out.data_ptr()) % 8 == 0 and (qkv.stride(0) | q_out.stride(0)) % 4 == 0, "rows of qkv and q_out must start at 8 bytes")
+    with _device(qkv):
+        check(kernels().loqa_rope_append8(
+            ptr(qkv), qkv.stride(0), ptr(cos_sin), 0 if cos_sin is None else cos_sin.shape[0], ptr(cache.k), ptr(cache.v), ptr(cache.k_scale),
+            ptr(cache.v_scale), ptr(cu_q), ptr(ctx_lens), ptr(block_tables), ptr(q_out), q_out.stride(0), T, B, H, G, D, cache.block_size,
+            cache.n_blocks, max_blocks, min(max_q, T), cache.kind, stream_ptr(qkv)), "rope_append8")
+    return q_out
+
+
+def read8(cache: Cache8, cu_k: torch.Tensor, first: torch.Tensor, block_tables: torch.Tensor, *, total: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cached rows as what they stand for: row cu_k[b] + i of the results, k and v [total, Hkv, D] bf16, is position
+    first[b] + i of sequence b (a prefix that moves to a bf16 cache, or is looked at). Zeros from pages that do not exist;
+    rows of no sequence are zeros too."""
+    B, max_blocks = _sequences(cu_k, first, block_tables, cache)
+    _need(0 <= total < 1 << 31, "total")
+    k, v = (torch.empty(total, cache.n_kv, cache.head_dim, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
+    if not cache.k.is_cuda:
+        return ref.read8(cache, cu_k, first, block_tables, k.zero_(), v.zero_())
+    if total == 0:
+        return k, v
+    if B == 0:
+        return k.zero_(), v.zero_()
+    with _device(k):
+        check(kernels().loqa_read8(ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale), ptr(cu_k), ptr(first), ptr(block_tables),
+                                   ptr(k), ptr(v), total, B, cache.n_kv, cache.head_dim, cache.block_size, cache.n_blocks, max_blocks,
+                                   cache.kind, stream_ptr(k)), "read8")
+    return k, v
+
+
+def attn8_parts(max_q: int, group: int, units: int, keys: int) -> int:
+    """Parts of a sequence's keys for ``units`` (sequence, kv head) pairs with at most ``keys`` keys."""
+    if max_q * group <= TOKEN_ROWS:
+        return max(1, min(-(-512 // units), -(-keys // 128), 64))
+    units *= -(-max_q * group // PROMPT_ROWS)
+    return max(1, min(512 // units, -(-keys // 256), 16))
+
+
+def attention8(q: torch.Tensor, cache: Cache8, cu_q: torch.Tensor, ctx_lens: torch.Tensor, block_tables: torch.Tensor, *, n_heads: int,
+               max_q: int, max_k: int | None = None, causal: bool = True, scale: float | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """Varlen attention off the 8-bit cache: token steps, prompts and prompt chunks behind cached tokens.
+
+    q: [T, >= H * D] bf16 (row stride may exceed H * D). Query i of a sequence of n rows sees the keys up to position
+    ctx - n + i (all ctx of them where not ``causal``). ``max_q`` bounds the rows of a sequence, ``max_k``
+    its context where the host knows a smaller bound than the block table's (it only chooses the split of the keys: in
+    how many parts they are summed up follows from the whole call). ``scale`` is 1 / sqrt(D) by default. Rows that see no
+    key give zeros. Returns [T, H * D] bf16 (``out`` where given)."""
+    H, G, D = n_heads, cache.n_kv, cache.head_dim
+    _need(H > 0 and H % G == 0, "n_heads must be a multiple of the cache's heads")
+    _need(max_q >= 0 and (max_k is None or max_k >= 0), "max_q and max_k")
+    _rows(q, H * D, "q", cache)
+    T = q.shape[0]
+    B, max_blocks = _sequences(cu_q, ctx_lens, block_tables, cache)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if out is None:
+        out = torch.empty(T, H * D, dtype=torch.bfloat16, device=q.device)
+    else:
+        _rows(out, H * D, "out", cache)
+        _need(out.shape[0] == T, "out has the rows of q")
+    if T == 0 or B == 0 or max_q == 0:
+        return out
+    if not q.is_cuda:
+        return ref.attention8(q, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, causal=causal, scale=scale, out=out)
+    keys = max_blocks * cache.block_size if max_k is None else min(max_k, max_blocks * cache.block_size)
+    max_q = min(max_q, T)
+    units = B * G
+    parts = attn8_parts(max_q, H // G, units, max(keys, 1))
+    st = stream_ptr(q)
+    ws = tickets = None
+    with _device(q):
+        if parts > 1:
+            rows = TOKEN_ROWS
+            if max_q * (H // G) > TOKEN_ROWS:
+                rows, units = PROMPT_ROWS, units * -(-max_q * (H // G) // PROMPT_ROWS)
+            ws, tickets = _sk_workspace(q.device, st, units * parts * rows * (D + 2), units)
+        check(kernels().loqa_attention8(
+            ptr(q), q.stride(0), ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale), ptr(cu_q), ptr(ctx_lens), ptr(block_tables),
+            ptr(out), out.stride(0), T, B, H, G, D, cache.block_size, cache.n_blocks, max_blocks, max_q, scale, int(causal), cache.kind, parts,
+            ptr(ws), 0 if ws is None else ws.numel(), ptr(tickets), 0 if tickets is None else tickets.numel(), st), "attention8")
+    return out
+
+
+# ------------------------------------------------------------------ pages of a step
+PAGE_STEP_SEQS = 4096
+
+
+class PageStep(NamedTuple):
+    """What a step's launches want of its sequences (int32 but for ``last_rows``): ``positions`` and ``slots`` [max_tokens]
+    (0 and -1 behind the last token), ``cu_q`` [B + 1], ``last_rows`` [B] int64 (the row of a sequence's last token, 0
+    where it has none), ``ctx_lens`` [B] with this step's tokens, ``ring`` [2], and ``status`` [1]: 0, or the sum of
+    1 (not enough free pages), 2 (more tokens than max_tokens), 4 (a sequence outgrows its table), 8 (numbers that no pool has)."""
+    cu_q: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    last_rows: torch.Tensor
+    ctx_lens: torch.Tensor
+    ring: torch.Tensor
+    status: torch.Tensor
+
+
+def page_step(new_lens: torch.Tensor, ctx_lens: torch.Tensor, block_tables: torch.Tensor, free_pages: torch.Tensor, ring: torch.Tensor, *,
+              block_size: int, max_tokens: int, ctx_out: torch.Tensor | None = None, ring_out: torch.Tensor | None = None) -> PageStep:
+    """The pages and slots of a step, on the GPU: what the host pool's ``step_meta`` does, for loops that never
+    come back to the host (a captured step whose lengths live on the GPU).
+
+    new_lens [B]: tokens of each sequence in this step (0: none; -1: the sequence has ended, and its pages go back);
+    ctx_lens [B]: its tokens before; block_tables [B, max_blocks]: its pages, to which new ones are added in place;
+    free_pages [N]: a ring of free pages, ``ring`` [2] = (place of the first, how many). Pages are taken in the order of the
+    sequences and given back behind the last free one. ``ctx_out`` / ``ring_out`` may be ``ctx_lens`` / ``ring`` themselves.
+    All or nothing: where the status is not 0, nothing changes and no token has a slot. At most 4096 sequences. A page that
+    several sequences share must not be given back here."""
+    _typed(block_tables, torch.int32, "block_tables")
+    for t, name in ((new_lens, "new_lens"), (ctx_lens, "ctx_lens"), (block_tables, "block_tables"), (free_pages, "free_pages"), (ring, "ring")):
+        _i32(t, name, block_tables)
+    B, pool = new_lens.numel(), free_pages.numel()
+    _need(0 < B <= PAGE_STEP_SEQS, f"1 to {PAGE_STEP_SEQS} sequences")
+    _need(ctx_lens.numel() == B and block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.shape[1] > 0, "ctx_lens [B], block_tables [B, max_blocks]")
+    _need(ring.numel() == 2 and pool > 0, "ring [2], free_pages [N]")
+    _need(block_size > 0 and block_size & (block_size - 1) == 0 and pool * block_size < 1 << 31, "block_size is a power of two, slots have 32 bits")
+    _need(0 <= max_tokens <= 1 << 30, "max_tokens")
+    dev, i32 = block_tables.device, torch.int32
+    if ctx_out is None:
+        ctx_out = torch.empty(B, dtype=i32, device=dev)
+    if ring_out is None:
+        ring_out = torch.empty(2, dtype=i32, device=dev)
+    for t, n, name in ((ctx_out, B, "ctx_out"), (ring_out, 2, "ring_out")):
+        _i32(t, name, block_tables)
+        _need(t.numel() == n, f"{name} has {n} entries")
+    step = PageStep(torch.empty(B + 1, dtype=i32, device=dev), torch.empty(max_tokens, dtype=i32, device=dev),
+                    torch.empty(max_tokens, dtype=i32, device=dev), torch.empty(B, dtype=torch.int64, device=dev), ctx_out, ring_out,
+                    torch.empty(1, dtype=i32, device=dev))
+    if not block_tables.is_cuda:
+        return ref.page_step(new_lens, ctx_lens, block_tables, free_pages, ring, block_size, step)
+    st = stream_ptr(block_tables)
+    with _device(block_tables):
+        _, tickets = _sk_workspace(dev, st, 1, 1)
+        check(kernels().loqa_page_step(
+            ptr(new_lens), ptr(ctx_lens), ptr(block_tables), ptr(free_pages), ptr(ring), ptr(step.cu_q), ptr(step.positions), ptr(step.slots),
+            ptr(step.last_rows), ptr(ctx_out), ptr(ring_out), ptr(step.status), ptr(tickets), B, block_tables.shape[1], block_size, pool,
+            max_tokens, st), "page_step")
+    return step
+
+
+# ------------------------------------------------------------------ 4-bit weights
+GROUPS = (32, 64, 128)
+
+
+def quantize4(w: torch.Tensor, group: int = 128, zeros: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """A matrix [N, K] in 4 bits, to nearest: (codes [N, K / 2] uint8, two a byte with the lower column in the lower half;
+    scales [N, K / group] bf16; zeros [N, K / group] uint8 or None: 8) with w ~ (code - zero) * scale."""
+    _need(w.dim() == 2 and group in GROUPS and w.shape[1] % group == 0, f"[N, K] with K a multiple of the group, one of {GROUPS}")
+    x = w.float().reshape(w.shape[0], -1, group)
+    z = None
+    if zeros:
+        lo, hi = x.amin(-1).clamp_max(0), x.amax(-1).clamp_min(0)
+        s = ((hi - lo) / 15).to(torch.bfloat16)
+        sf = torch.where(s > 0, s, torch.ones_like(s)).float()
+        z = (-lo / sf).round().clamp(0, 15).to(torch.uint8)
+        c = (x / sf[..., None]).round() + z[..., None]
+    else:
+        s = (x.abs().amax(-1) / 7).to(torch.bfloat16)
+        sf = torch.where(s > 0, s, torch.ones_like(s)).float()
+        c = (x / sf[..., None]).round() + 8
+    c = c.clamp(0, 15).to(torch.uint8).reshape(w.shape)
+    return c[:, 0::2] | c[:, 1::2] << 4, s, z
+
+
+class Weight4:
+    """A weight matrix [N, K] in 4 bits for :func:`linear4`: codes, scales and zeros as :func:`quantize4` returns them
+    (zeros up to 15; group 32, 64 or 128 by their shapes), laid out once for the kernel. The tensors given are not kept on the GPU."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None):
+        _typed(codes, torch.uint8, "codes")
+        _typed(scales, torch.bfloat16, "scales")
+        _need(codes.dim() == 2 and scales.dim() == 2 and scales.shape[0] == codes.shape[0], "codes [N, K / 2], scales [N, K / group]")
+        self.n, self.k = codes.shape[0], codes.shape[1] * 2
+        groups = scales.shape[1]
+        _need(self.n > 0 and groups > 0 and self.k % groups == 0 and self.k // groups in GROUPS, f"groups of {GROUPS}")
+        self.group = self.k // groups
+        if zeros is not None:
+            _typed(zeros, torch.uint8, "zeros")
+            _need(zeros.shape == scales.shape, "zeros have the shape of scales")
+        _need(all(t is None or t.device == codes.device for t in (scales, zeros)), "tensors of one device")
+        self.device = codes.device
+        codes, scales = codes.contiguous(), scales.contiguous()
+        zeros = None if zeros is None else zeros.contiguous()
+        if not codes.is_cuda:
+            self.codes, self.scales, self.zeros = codes, scales, zeros
+            return
+        tiles, blocks = -(-self.n // 16), -(-self.k // 128)
+        self.codes = torch.empty(tiles * blocks * 256, dtype=torch.int32, device=codes.device)
+        self.scales = torch.empty(tiles * groups * 16, dtype=torch.bfloat16, device=codes.device)
+        self.zeros = None if zeros is None else torch.empty(tiles * groups * 16, dtype=torch.uint8, device=codes.device)
+        with _device(codes):
+            check(kernels().loqa_shuffle4(ptr(codes), ptr(scales), ptr(zeros), ptr(self.codes), ptr(self.scales), ptr(self.zeros), self.n, self.k,
+                                          self.group, stream_ptr(codes)), "shuffle4")
+
+    @classmethod
+    def quantize(cls, w: torch.Tensor, group: int = 128, zeros: bool = False) -> "Weight4":
+        return cls(*quantize4(w, group, zeros))
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zeros) if t is not None)
+
+
+def linear4(x: torch.Tensor, w: Weight4, b: torch.Tensor | None = None) -> torch.Tensor:
+    """x [..., K] bf16 times the transpose of a 4-bit weight (+ bias [N] bf16): [..., N] bf16, summed up in f32. Made for
+    the few rows of token steps; more than 64 read the weight again for every 64. An infinite or NaN entry of x makes its row NaN."""
+    _typed(x, torch.bfloat16, "x")
+    _need(x.dim() >= 1 and x.shape[-1] == w.k, f"x has {w.k} columns")
+    _need(x.device == w.device, f"x must be on {w.device}")
+    if b is not None:
+        _typed(b, torch.bfloat16, "b")
+        _need(b.shape == (w.n,) and b.is_contiguous() and b.device == w.device, f"b is [{w.n}], contiguous")
+    if not x.is_cuda:
+        return ref.linear4(x, w, b)
+    y = torch.empty(*x.shape[:-1], w.n, dtype=torch.bfloat16, device=x.device)
+    x2 = x if x.dim() == 2 else x.reshape(-1, w.k)
+    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < 0 or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    M = x2.shape[0]
+    if M == 0:
+        return y
+    with _device(x):
+        check(kernels().loqa_linear4(ptr(x2), x2.stride(0), ptr(w.codes), ptr(w.scales), ptr(w.zeros), ptr(b), ptr(y), w.n, M, w.n, w.k, w.group,
+                                     stream_ptr(x)), "linear4")
+    return y

@@ -1428,3 +1428,152 @@ def retention_prep(u, H: int, D: int, Dv: int, cos_sin, dims: int, positions):
         q, k = rotate_pairs(q, cs, dims), rotate_pairs(k, cs, dims)
     return torch.cat([q.reshape(T, H * D), k.reshape(T, H * D) * D ** -0.5,
                       u[:, 2 * H * D:2 * H * D + H * Dv].float()], dim=1).contiguous()
+
+
+# --------------------------------------------------------------- low bits (ops.lowbit)
+_CODES_MOST = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+SCALE_LEAST = 2.0 ** -100
+
+
+def page_scale8(top, dtype):
+    """Scale of a page whose largest magnitude is ``top``: top / 127, or for e4m3 the power of two from top / 448 on."""
+    s = top / _CODES_MOST[dtype]
+    if dtype is torch.int8:
+        return s
+    m, e = torch.frexp(s)
+    return torch.where(torch.isfinite(s) & (s > 0), torch.ldexp(torch.ones_like(s), torch.where(m > 0.5, e, e - 1)), s)
+
+
+def codes8(x, dtype):
+    """x (already over its scale) to the nearest code; what is no number becomes the largest."""
+    most = _CODES_MOST[dtype]
+    x = torch.nan_to_num(x, nan=most, posinf=most, neginf=-most).clamp(-most, most)
+    return x.round().to(torch.int8) if dtype is torch.int8 else x.to(dtype)
+
+
+def _feeds(cu_q, T, max_q):
+    cu = [min(max(c, 0), T) for c in cu_q.tolist()]
+    return [(a, min(max(b - a, 0), max_q), max(b - a, 0)) for a, b in zip(cu, cu[1:])]
+
+
+def rope_append8(qkv, cos_sin, cache, cu_q, ctx_lens, block_tables, *, n_heads, max_q, q_out):
+    H, G, D, P = n_heads, cache.n_kv, cache.head_dim, cache.block_size
+    dtype, ctx = cache.k.dtype, ctx_lens.tolist()
+    for b, (q0, n, fed) in enumerate(_feeds(cu_q, qkv.shape[0], max_q)):
+        if n == 0:
+            continue
+        start = ctx[b] - fed
+        end = start + n
+        x = qkv[q0:q0 + n, :(H + 2 * G) * D].float().reshape(n, H + 2 * G, D)
+        qk, v = x[:, :H + G], x[:, H + G:]
+        if cos_sin is not None:
+            qk = apply_rope(qk, cos_sin[(torch.arange(n) + start).clamp(0, cos_sin.shape[0] - 1)])
+        q_out[q0:q0 + n, :H * D] = qk[:, :H].reshape(n, H * D).to(q_out.dtype)
+        for p in range(max(start, 0) // P * P, end, P):
+            if p // P >= block_tables.shape[1]:
+                break
+            page = int(block_tables[b, p // P])
+            if not 0 <= page < cache.n_blocks:
+                continue
+            lo, hi = max(start, p), min(end, p + P)
+            off = lo - p
+            for codes, scale, new in ((cache.k, cache.k_scale, qk[:, H:]), (cache.v, cache.v_scale, v)):
+                rows = new[lo - start:hi - start].transpose(0, 1)              # [G, rows, D]
+                had = scale[page].clone()
+                now = torch.maximum(page_scale8(rows.abs().amax((1, 2)), dtype), had if off else torch.zeros_like(had))
+                now = torch.where(now < SCALE_LEAST, torch.full_like(now, SCALE_LEAST), now)
+                if off:
+                    old = codes8(codes[page, :, :off].float() * had[:, None, None] / now[:, None, None], dtype)
+                    grown = (now != had).view(-1, 1, 1)
+                    codes[page, :, :off] = torch.where(grown, old.float(), codes[page, :, :off].float()).to(dtype)
+                codes[page, :, off:off + hi - lo] = codes8(rows / now[:, None, None], dtype)
+                scale[page] = now
+    return q_out
+
+
+def read8(cache, cu_k, first, block_tables, k, v):
+    P = cache.block_size
+    for b, (at, n, _) in enumerate(_feeds(cu_k, k.shape[0], k.shape[0])):
+        for i in range(n):
+            pos = int(first[b]) + i
+            page = int(block_tables[b, pos // P]) if 0 <= pos < P * block_tables.shape[1] else -1
+            if 0 <= page < cache.n_blocks:
+                k[at + i] = (cache.k[page, :, pos % P].float() * cache.k_scale[page][:, None]).to(k.dtype)
+                v[at + i] = (cache.v[page, :, pos % P].float() * cache.v_scale[page][:, None]).to(v.dtype)
+    return k, v
+
+
+def attention8(q, cache, cu_q, ctx_lens, block_tables, *, n_heads, max_q, causal, scale, out):
+    H, G, D, P = n_heads, cache.n_kv, cache.head_dim, cache.block_size
+    for b, (q0, n, fed) in enumerate(_feeds(cu_q, q.shape[0], max_q)):
+        if n == 0:
+            continue
+        ctx = int(ctx_lens[b])
+        L = min(max(ctx, 0), P * block_tables.shape[1])
+        pos = torch.arange(L)
+        pages = block_tables[b].long()[pos // P]
+        there = (pages >= 0) & (pages < cache.n_blocks)
+        pages = torch.where(there, pages, 0)
+        k, v = (torch.where(there[:, None, None], codes[pages, :, pos % P].float() * s[pages].clamp_min(SCALE_LEAST)[..., None], 0.0)
+                for codes, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+        x = q[q0:q0 + n, :H * D].float().reshape(n, H, D)
+        w = torch.einsum("ihd,jhd->hij", x, k.repeat_interleave(H // G, 1)) * scale
+        hide = ~there[None, :].expand(n, L)
+        if causal:
+            hide = hide | (pos[None] > (ctx - fed + torch.arange(n))[:, None])
+        w = w.masked_fill(hide[None], -math.inf)
+        top = w.amax(-1, keepdim=True) if L else w.new_zeros(H, n, 1)
+        e = torch.exp(w - torch.where(top == -math.inf, torch.zeros_like(top), top))
+        total = e.sum(-1, keepdim=True)
+        p = e / torch.where(total == 0, torch.ones_like(total), total)
+        out[q0:q0 + n, :H * D] = torch.einsum("hij,jhd->ihd", p, v.repeat_interleave(H // G, 1)).reshape(n, H * D).to(out.dtype)
+    return out
+
+
+def page_step(new_lens, ctx_lens, block_tables, free_pages, ring, block_size, step):
+    P, (B, width), pool = block_size, block_tables.shape, free_pages.numel()
+    new, ctx, (head, count), most = new_lens.tolist(), ctx_lens.tolist(), ring.tolist(), step.slots.numel()
+    want = [-(-(c + max(n, 0)) // P) - -(-c // P) for n, c in zip(new, ctx)]
+    back = [-(-c // P) if n == -1 else 0 for n, c in zip(new, ctx)]
+    fed = [max(n, 0) for n in new]
+    status = (1 if sum(want) > count else 0) | (2 if sum(fed) > most else 0) | (4 if any(c + n > width * P for c, n in zip(ctx, fed)) else 0)
+    if min(new) < -1 or min(ctx) < 0 or not 0 <= head < pool or not 0 <= count <= pool or count + sum(back) > pool:
+        status |= 8
+    step.positions.zero_()
+    step.slots.fill_(-1)
+    step.last_rows.zero_()
+    step.status.fill_(status)
+    if status:
+        step.cu_q.zero_()
+        step.ctx_lens.copy_(ctx_lens)
+        step.ring.copy_(ring)
+        return step
+    at, first, given, free = 0, 0, 0, free_pages.tolist()
+    step.cu_q[0] = 0
+    for i, (n, c) in enumerate(zip(fed, ctx)):
+        held = -(-c // P)
+        for j in range(want[i]):
+            block_tables[i, held + j] = free[(head + first + j) % pool]
+        for j in range(back[i]):
+            free_pages[(head + count + given + j) % pool] = block_tables[i, j]
+        pos = torch.arange(c, c + n)
+        step.positions[at:at + n] = pos.to(torch.int32)
+        step.slots[at:at + n] = (block_tables[i].long()[pos // P] * P + pos % P).to(torch.int32)
+        at, first, given = at + n, first + want[i], given + back[i]
+        step.cu_q[i + 1] = at
+        if n:
+            step.last_rows[i] = at - 1
+    step.ctx_lens.copy_(torch.tensor([0 if n == -1 else c + f for n, c, f in zip(new, ctx, fed)], dtype=torch.int32))
+    step.ring.copy_(torch.tensor([(head + first) % pool, count - first + given], dtype=torch.int32))
+    return step
+
+
+def dense4(codes, scales, zeros):
+    """The matrix [N, K] f32 that codes [N, K / 2], scales and zeros stand for."""
+    c = torch.stack([codes & 15, codes >> 4], -1).reshape(*scales.shape, -1).float()
+    return ((c - (8.0 if zeros is None else zeros.float()[..., None])) * scales.float()[..., None]).reshape(codes.shape[0], -1)
+
+
+def linear4(x, w, b=None):
+    y = x.float() @ dense4(w.codes, w.scales, w.zeros).t()
+    return (y if b is None else y + b.float()).to(x.dtype)
