@@ -12,6 +12,8 @@
 #include "cache8.h"
 #include "flash_pipe.h"
 
+#define A8_NONE -3.0e38f                           // a row's maximum before its first key
+
 struct Attn8Args {
   const bf16_t* q;
   long long ldq;
@@ -22,7 +24,7 @@ struct Attn8Args {
   long long ldo;
   float* ws;                             // partials: [unit][part][rows][D + 2]
   int* tickets;
-  int T, H, G, sh, n_blocks, max_blocks, max_q, parts, causal, row_blocks;
+  int T, B, H, G, sh, n_blocks, max_blocks, max_q, parts, causal, row_blocks, fold;
   float scale_log2;
 };
 
@@ -95,7 +97,7 @@ __device__ __forceinline__ void a8_join(const Attn8Args& A, size_t unit, int n, 
   const auto rs = __builtin_amdgcn_make_buffer_rsrc(A.ws + unit * A.parts * R * (D + 2), 0, A.parts * PER, 0x00020000);
   for (int id = threadIdx.x; id < rows * (D / 4); id += NT) {
     const int r = id / (D / 4), c = id % (D / 4) * 4;
-    float ms = -1e30f, l = 0.f;
+    float ms = A8_NONE, l = 0.f;
     float4v o = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < n; s0 += OB) {
       float4v v[OB];
@@ -253,7 +255,7 @@ __global__ __launch_bounds__(A8_WAVES * 64) void attn8_token_kernel(Attn8Args A)
   float4v acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = float4v{0.f, 0.f, 0.f, 0.f};
-  float m_run = -1e30f, l_run = 0.f;
+  float m_run = A8_NONE, l_run = 0.f;
   int pages[2][2] = {{page_at(kt0, 0), page_at(kt0, 1)}, {page_at(kt0 + STEP, 0), page_at(kt0 + STEP, 1)}};
   ask(kt0, ring, pages[0]);
   ask(kt0 + STEP, ring + L::STAGE, pages[1]);
@@ -381,15 +383,20 @@ template <int D> struct A8Prompt {
 };
 
 template <int D, int KIND>
-__global__ __launch_bounds__(256) void attn8_prompt_kernel(Attn8Args A) {
+__global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   using L = A8Prompt<D>;
   constexpr int NS = D / 16, NDT = D / 32, CH = D / 16, N = A8P_KEYS * CH / 256;    // chunks of 16 codes a row, a thread
   static_assert(N * 256 == A8P_KEYS * CH, "whole chunks a thread");
   __shared__ __attribute__((aligned(1024))) unsigned char lds[L::SMEM];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, li = lane & 15;
-  const int b = blockIdx.z / A.parts, part = blockIdx.z - b * A.parts, kvh = blockIdx.y, Gq = A.H / A.G;
+  // (sequence, kv head) from the workgroup's number modulo as many, so that a head's workgroups share an XCD's L2 where these are a
+  // multiple of eight; blocks of rows from the longest down, but the second of two workgroups a compute unit from the
+  // shortest up: with all of them on the chip at once, a long and a short one share it
+  const int b = blockIdx.x / A.G % A.B, kvh = blockIdx.x % A.G, Gq = A.H / A.G;
+  const int rest = blockIdx.x / A.G / A.B, part = rest % A.parts, turn = rest / A.parts;
   const A8Feed f = a8_feed(A, b);
-  const int block = A.row_blocks - 1 - (int)blockIdx.x;      // the longest first
+  const int half = (A.row_blocks + 1) / 2;
+  const int block = A.fold && turn >= half ? turn - half : A.row_blocks - 1 - turn;
   const int r0 = block * A8P_ROWS, rows = min(f.n * Gq - r0, A8P_ROWS);
   if (rows <= 0) return;
   // keys that some row of the block sees, in parts of whole tiles
@@ -420,41 +427,46 @@ __global__ __launch_bounds__(256) void attn8_prompt_kernel(Attn8Args A) {
     }
     top = fl_max32(top);
     const int e = a8_lift(top);
-    factor = ldexpf(A.scale_log2, -e);
+    factor = ldexpf(fabsf(A.scale_log2), -e);
+    const float sign = A.scale_log2 < 0.f ? -1.f : 1.f;      // a factor above zero keeps a group's largest product its largest score
 #pragma unroll
     for (int u = 0; u < NS; ++u)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) qf[u][i] = (_Float16)ldexpf(x[u][i], e);
+      for (int i = 0; i < 8; ++i) qf[u][i] = (_Float16)(sign * ldexpf(x[u][i], e));
   }
 
   // this thread's chunks: row tid / CH + i 256 / CH of the tile
   const int cr = tid / CH, cc = tid % CH;
+  // Codes are asked for a tile ahead and their pages' numbers two, so that no load waits for another one.
+  const int last = max(f.keys - 1, 0);
   uint4 kw[N], vw[N];
+  int pages[N], group_page = 0;
   float sk = 0.f, sv = 0.f;
   bool there = false;
+  auto look = [&](int tile) {
+    const int kt = tile * A8P_KEYS;
+#pragma unroll
+    for (int i = 0; i < N; ++i) pages[i] = bt[min(kt + cr + i * (256 / CH), last) >> A.sh];
+    group_page = bt[min(kt + 16 * (tid & 3), last) >> A.sh];
+  };
   auto fetch = [&](int tile) {
     const int kt = tile * A8P_KEYS;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int key = kt + cr + i * (256 / CH);
-      kw[i] = vw[i] = make_uint4(0, 0, 0, 0);
-      if (key < f.keys) {
-        const int page = bt[key >> A.sh];
-        if ((unsigned)page < (unsigned)A.n_blocks) {
-          const size_t off = ((((size_t)page * A.G + kvh) << A.sh) + (key & ((1 << A.sh) - 1))) * D + cc * 16;
-          kw[i] = *reinterpret_cast<const uint4*>(A.k + off);
-          vw[i] = *reinterpret_cast<const uint4*>(A.v + off);
-        }
+      const int key = min(kt + cr + i * (256 / CH), last);
+      const bool ok = (unsigned)pages[i] < (unsigned)A.n_blocks;
+      const size_t off = ((((size_t)(ok ? pages[i] : 0) * A.G + kvh) << A.sh) + (key & ((1 << A.sh) - 1))) * D + cc * 16;
+      kw[i] = *reinterpret_cast<const uint4*>(A.k + off);
+      vw[i] = *reinterpret_cast<const uint4*>(A.v + off);
+      if (__any(!ok || kt + cr + i * (256 / CH) > last)) {   // codes that are none may be NaN, which no weight of zero hides
+        if (!ok || kt + cr + i * (256 / CH) > last) kw[i] = vw[i] = make_uint4(0, 0, 0, 0);
       }
     }
     if (tid < 4) {                                           // the scales of 16 keys
-      const int key = kt + 16 * tid;
-      there = false;
-      if (key < f.keys) {
-        const int page = bt[key >> A.sh];
-        there = (unsigned)page < (unsigned)A.n_blocks;
-        if (there) { sk = A.ks[(size_t)page * A.G + kvh]; sv = A.vs[(size_t)page * A.G + kvh]; }
-      }
+      there = (unsigned)group_page < (unsigned)A.n_blocks;
+      const size_t at = (size_t)(there ? group_page : 0) * A.G + kvh;
+      sk = A.ks[at];
+      sv = A.vs[at];
     }
   };
   auto store = [&](int stage) {
@@ -472,7 +484,7 @@ __global__ __launch_bounds__(256) void attn8_prompt_kernel(Attn8Args A) {
     if (tid < 4) {
       float* s = reinterpret_cast<float*>(lds + L::SCALES + stage * 64) + tid;
       const float vs = a8_least(sv);
-      s[0] = there ? sk : 0.f;
+      s[0] = there ? a8_least(sk) : 1.f;
       s[4] = there ? __builtin_amdgcn_logf(vs) : -INFINITY;
       s[8] = there ? 1.f / vs : 0.f;
     }
@@ -489,14 +501,19 @@ __global__ __launch_bounds__(256) void attn8_prompt_kernel(Attn8Args A) {
   float16v acc[NDT];
 #pragma unroll
   for (int d = 0; d < NDT; ++d) acc[d] = zero;
-  float m = -1e30f, l = 0.f;
+  float m = A8_NONE, l = 0.f;
   if (n > 0) {
+    look(i0);
     fetch(i0);
+    look(i0 + 1);
     store(0);
   }
   for (int i = 0; i < n; ++i) {
     const int stage = i & 1, kt = (i0 + i) * A8P_KEYS;
-    if (i + 1 < n) fetch(i0 + i + 1);
+    if (i + 1 < n) {
+      fetch(i0 + i + 1);
+      look(i0 + i + 2);
+    }
     __syncthreads();                                         // this stage is written; nobody reads the other one any more
     float16v s[2] = {zero, zero};
 #pragma unroll
@@ -505,55 +522,60 @@ __global__ __launch_bounds__(256) void attn8_prompt_kernel(Attn8Args A) {
       for (int t = 0; t < 2; ++t)
         s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*fl_lds<c8_h8>(kb[u] + stage * L::STAGE + 32 * t * D * 2), qf[u], s[t], 0, 0, 0);
     const float* sc = reinterpret_cast<const float*>(lds + L::SCALES + stage * 64);
-    float mx = -INFINITY;
-    const bool edge = kt + A8P_KEYS > f.keys || (A.causal && kt + A8P_KEYS - 1 > f.past + (r0 + wave * 32) / Gq);
+    if (kt + A8P_KEYS > f.keys || (A.causal && kt + A8P_KEYS - 1 > f.past + (r0 + wave * 32) / Gq)) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const float c = factor * sc[2 * t + g], lv = sc[4 + 2 * t + g];
-#pragma unroll
-        for (int j = 8 * g; j < 8 * g + 8; ++j) {
-          float x = fmaf(s[t][j], c, lv);
-          if (edge) {
-            const int key = kt + 32 * t + (j & 3) + 8 * (j >> 2) + 4 * h;
-            if (key >= f.keys || key > qpos) x = -INFINITY;
-          }
-          s[t][j] = x;
-          mx = fmaxf(mx, x);
+        for (int j = 0; j < 16; ++j) {
+          const int key = kt + 32 * t + (j & 3) + 8 * (j >> 2) + 4 * h;
+          if (key >= f.keys || key > qpos) s[t][j] = -INFINITY;
         }
+    }
+    // t = x c + log2 vs with c above zero: the largest product of a group of 16 keys is its largest score
+    float c[4], lv[4], mx = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float k = factor * sc[g];
+      c[g] = k < 1.1754943508222875e-38f ? 1.1754943508222875e-38f : k;     // of no use to a masked -infinity if zero; NaN stays
+      lv[g] = sc[4 + g];
+      float x = s[g >> 1][8 * (g & 1)];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) x = fmaxf(x, s[g >> 1][8 * (g & 1) + j]);
+      mx = fmaxf(mx, fmaf(x, c[g], lv[g]));
+    }
+    const float m_new = fmaxf(m, fl_max32(mx));
+    if (__any(m_new > m)) {
+      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < NDT; ++d)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[d][j] *= alpha;
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      c8_h8 p;
+      float sum = 0.f;
+      const float off = lv[g] - m;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j], c[g], off));
+        sum += e;
+        p[j] = (_Float16)e;
       }
-    const float m_new = fmaxf(m, fl_max32(mx)), alpha = exp2f(m - m_new);
-    m = m_new;
-    l *= alpha;
+      l = fmaf(sum, sc[8 + g], l);
 #pragma unroll
-    for (int d = 0; d < NDT; ++d)
+      for (int d = 0; d < NDT; ++d) {
+        const unsigned a = vb[d] + stage * L::STAGE + 16 * g * D * 2;
+        const fl_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a));
+        const fl_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a + 8 * D * 2));
+        short8 a8;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) acc[d][j] *= alpha;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        c8_h8 p;
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float e = exp2f(s[t][8 * g + j] - m_new);
-          sum += e;
-          p[j] = (_Float16)e;
-        }
-        l = fmaf(sum, sc[8 + 2 * t + g], l);
-#pragma unroll
-        for (int d = 0; d < NDT; ++d) {
-          const unsigned a = vb[d] + stage * L::STAGE + (32 * t + 16 * g) * D * 2;
-          const fl_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a));
-          const fl_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a + 8 * D * 2));
-          short8 a8;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) { a8[j] = lo[j]; a8[4 + j] = hi[j]; }
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(c8_h8, a8), p, acc[d], 0, 0, 0);
-        }
+        for (int j = 0; j < 4; ++j) { a8[j] = lo[j]; a8[4 + j] = hi[j]; }
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(c8_h8, a8), p, acc[d], 0, 0, 0);
       }
+    }
     if (i + 1 < n) store(1 - stage);
   }
   l = fl_both32(l);                                          // a lane has summed up its half of the keys
@@ -594,12 +616,13 @@ extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const voi
   const bool token = (long long)max_q * (H / G) <= A8_ROWS;
   const long long blocks = token ? 1 : ((long long)max_q * (H / G) + A8P_ROWS - 1) / A8P_ROWS, units = (long long)B * G * blocks;
   const int rows = token ? A8_ROWS : A8P_ROWS;
-  if (G > 65535 || (token ? B : (long long)B * parts) > 65535 || blocks > 1 << 24 || (long long)parts * rows * (D + 2) * 4 >= 1LL << 31)
+  if (token ? G > 65535 || B > 65535 || parts > 1 << 24 : units * parts > 1 << 30) return (int)hipErrorInvalidValue;
+  if (blocks > 1 << 24 || (long long)parts * rows * (D + 2) * 4 >= 1LL << 31)
     return (int)hipErrorInvalidValue;
   if (parts > 1 && (!ws || !tickets || ws_floats < units * parts * rows * (D + 2) || n_tickets < units)) return (int)hipErrorInvalidValue;
   const Attn8Args a{(const bf16_t*)q, ldq, (const unsigned char*)k, (const unsigned char*)v, (const float*)ks, (const float*)vs, (const int*)cu,
-                    (const int*)ctx, (const int*)bt, (bf16_t*)out, ldo, (float*)ws, (int*)tickets, T, H, G, __builtin_ctz(blk), n_blocks, max_blocks,
-                    max_q, parts, causal, (int)blocks, scale * 1.4426950408889634f};
+                    (const int*)ctx, (const int*)bt, (bf16_t*)out, ldo, (float*)ws, (int*)tickets, T, B, H, G, __builtin_ctz(blk), n_blocks, max_blocks,
+                    max_q, parts, causal, (int)blocks, units * parts <= 512, scale * 1.4426950408889634f};
   if (token) {
     const dim3 grid(parts, G, B);
 #define GO(D_, K_) hipLaunchKernelGGL((attn8_token_kernel<D_, K_>), grid, dim3(A8_WAVES * 64), 0, st, a)
@@ -607,7 +630,7 @@ extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const voi
     else { if (kind == C8_INT8) GO(128, C8_INT8); else GO(128, C8_E4M3); }
 #undef GO
   } else {
-    const dim3 grid((unsigned)blocks, G, B * parts);
+    const dim3 grid((unsigned)(units * parts));
 #define GO(D_, K_) hipLaunchKernelGGL((attn8_prompt_kernel<D_, K_>), grid, dim3(256), 0, st, a)
     if (D == 64) { if (kind == C8_INT8) GO(64, C8_INT8); else GO(64, C8_E4M3); }
     else { if (kind == C8_INT8) GO(128, C8_INT8); else GO(128, C8_E4M3); }
