@@ -24,7 +24,7 @@ struct Attn8Args {
   long long ldo;
   float* ws;                             // partials: [unit][part][rows][D + 2]
   int* tickets;
-  int T, B, H, G, sh, n_blocks, max_blocks, max_q, parts, causal, row_blocks, fold;
+  int T, B, H, G, sh, n_blocks, max_blocks, max_q, parts, causal, row_blocks, each;
   float scale_log2;
 };
 
@@ -43,13 +43,43 @@ __device__ __forceinline__ A8Feed a8_feed(const Attn8Args& A, int b) {
 
 __device__ __forceinline__ float a8_least(float s) { return s < C8_LEAST ? C8_LEAST : s; }   // NaN stays
 
-// eight entries of a query row in f32 (bf16 at any 2-byte place), zeros for a row that is none
-__device__ __forceinline__ void a8_row8(const bf16_t* p, bool whole, float* f) {
-  if (whole) {
-    unpack8(*reinterpret_cast<const uint4*>(p), f);
+// N pieces of eight entries of a query row, piece u at at(u), asked for together (rows at odd places entry by entry)
+template <int N, typename At> __device__ __forceinline__ void a8_row(const Attn8Args& A, uint4 (&x)[N], At&& at) {
+  if ((((size_t)A.q | (size_t)A.ldq * 2) & 15) == 0) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) x[u] = *reinterpret_cast<const uint4*>(at(u));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = bf2f(p[i]);
+    for (int u = 0; u < N; ++u) {
+      const bf16_t* p = at(u);
+      unsigned w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = p[2 * i] | (unsigned)p[2 * i + 1] << 16;
+      x[u] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// the f16 form of a row's pieces, times 2^e and its sign; top: the row's largest magnitude
+template <int N> __device__ __forceinline__ float a8_top(const uint4 (&x)[N]) {
+  float top = 0.f;
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    float f[8];
+    unpack8(x[u], f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(f[i]));
+  }
+  return top;
+}
+template <int N> __device__ __forceinline__ void a8_queries(const uint4 (&x)[N], bool row, int e, bool minus, c8_h8 (&q)[N]) {
+  const float by = !row ? 0.f : ldexpf(minus ? -1.f : 1.f, e);
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    float f[8];
+    unpack8(x[u], f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[u][i] = row ? (_Float16)(f[i] * by) : (_Float16)0.f;
   }
 }
 
@@ -193,27 +223,16 @@ __global__ __launch_bounds__(A8_WAVES * 64) void attn8_token_kernel(Attn8Args A)
   c8_h8 qf[2 * NS];
   float factor;
   {
-    const bool row = li < rows, whole = (((size_t)A.q | (size_t)A.ldq * 2) & 15) == 0;
-    const bf16_t* qp = A.q + (size_t)(f.q0 + tok) * A.ldq + (size_t)(kvh * Gq + li - tok * Gq) * D + 16 * fq;
-    float x[2 * NS][8];
-    float top = 0.f;
-#pragma unroll
-    for (int u = 0; u < 2 * NS; ++u) {
-      if (row) a8_row8(qp + u / 2 * 64 + u % 2 * 8, whole, x[u]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (!row) x[u][i] = 0.f;
-        top = fmaxf(top, fabsf(x[u][i]));
-      }
-    }
+    const bool row = li < rows;
+    const bf16_t* qp = A.q + (size_t)(f.q0 + (row ? tok : 0)) * A.ldq + (size_t)(kvh * Gq + (row ? li - tok * Gq : 0)) * D + 16 * fq;
+    uint4 x[2 * NS];
+    a8_row(A, x, [&](int u) { return qp + u / 2 * 64 + u % 2 * 8; });
+    float top = a8_top(x);
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const int e = a8_lift(top);
     factor = ldexpf(A.scale_log2, -e);
-#pragma unroll
-    for (int u = 0; u < 2 * NS; ++u)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) qf[u][i] = (_Float16)ldexpf(x[u][i], e);
+    a8_queries(x, row, e, false, qf);
 #pragma unroll
     for (int u = 0; u < 2 * NS; ++u) asm volatile("" : "+v"(qf[u]));   // here before the loads whose count the compiler does not know
     asm volatile("" : "+v"(factor));
@@ -379,6 +398,7 @@ __global__ __launch_bounds__(A8_WAVES * 64) void attn8_token_kernel(Attn8Args A)
 
 template <int D> struct A8Prompt {
   static constexpr int K = A8P_KEYS * D * 2, STAGE = 2 * K;
+  static_assert((STAGE & (STAGE - 1)) == 0, "stages differ in one bit of an address, the array starts at a multiple of both");
   static constexpr int SCALES = 2 * STAGE, SMEM = 2 * STAGE + 2 * 64;    // [stage][ks 4, log2 vs 4, 1 / vs 4]
 };
 
@@ -387,24 +407,21 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   using L = A8Prompt<D>;
   constexpr int NS = D / 16, NDT = D / 32, CH = D / 16, N = A8P_KEYS * CH / 256;    // chunks of 16 codes a row, a thread
   static_assert(N * 256 == A8P_KEYS * CH, "whole chunks a thread");
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[L::SMEM];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, li = lane & 15;
+  __shared__ __attribute__((aligned(2 * L::STAGE))) unsigned char lds[L::SMEM];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, li = lane & 15;
   // (sequence, kv head) from the workgroup's number modulo as many, so that a head's workgroups share an XCD's L2 where these are a
-  // multiple of eight; blocks of rows from the longest down, but the second of two workgroups a compute unit from the
-  // shortest up: with all of them on the chip at once, a long and a short one share it
+  // multiple of eight; blocks of rows from the longest down
   const int b = blockIdx.x / A.G % A.B, kvh = blockIdx.x % A.G, Gq = A.H / A.G;
   const int rest = blockIdx.x / A.G / A.B, part = rest % A.parts, turn = rest / A.parts;
   const A8Feed f = a8_feed(A, b);
-  const int half = (A.row_blocks + 1) / 2;
-  const int block = A.fold && turn >= half ? turn - half : A.row_blocks - 1 - turn;
+  const int block = A.row_blocks - 1 - turn;
   const int r0 = block * A8P_ROWS, rows = min(f.n * Gq - r0, A8P_ROWS);
   if (rows <= 0) return;
   // keys that some row of the block sees, in parts of whole tiles
   const int seen = A.causal ? min(f.keys, max(f.past + (r0 + rows - 1) / Gq + 1, 0)) : f.keys;
-  const int tiles = (seen + A8P_KEYS - 1) / A8P_KEYS, each = max((tiles + A.parts - 1) / A.parts, 1);
-  const int nparts = max((tiles + each - 1) / each, 1);
+  const int tiles = (seen + A8P_KEYS - 1) / A8P_KEYS, nparts = min(max((tiles + A.each - 1) / A.each, 1), A.parts);
   if (part >= nparts) return;
-  const int i0 = part * each, n = min(tiles, i0 + each) - i0;
+  const int i0 = (int)((long long)tiles * part / nparts), n = (int)((long long)tiles * (part + 1) / nparts) - i0;
   const unsigned base = fl_lds_at(lds);
   const int* bt = A.bt + (size_t)b * A.max_blocks;
 
@@ -412,55 +429,44 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   c8_h8 qf[NS];
   float factor;
   {
-    const bool row = r < r0 + rows, whole = (((size_t)A.q | (size_t)A.ldq * 2) & 15) == 0;
+    const bool row = r < r0 + rows;
     const bf16_t* qp = A.q + (size_t)(f.q0 + tok) * A.ldq + (size_t)(kvh * Gq + r % Gq) * D + 8 * h;
-    float top = 0.f;
-    float x[NS][8];
-#pragma unroll
-    for (int u = 0; u < NS; ++u) {
-      if (row) a8_row8(qp + 16 * u, whole, x[u]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (!row) x[u][i] = 0.f;
-        top = fmaxf(top, fabsf(x[u][i]));
-      }
-    }
-    top = fl_max32(top);
-    const int e = a8_lift(top);
-    factor = ldexpf(fabsf(A.scale_log2), -e);
-    const float sign = A.scale_log2 < 0.f ? -1.f : 1.f;      // a factor above zero keeps a group's largest product its largest score
-#pragma unroll
-    for (int u = 0; u < NS; ++u)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) qf[u][i] = (_Float16)(sign * ldexpf(x[u][i], e));
+    uint4 x[NS];
+    a8_row(A, x, [&](int u) { return qp + 16 * u; });
+    const int e = a8_lift(fl_max32(a8_top(x)));
+    factor = ldexpf(fabsf(A.scale_log2), -e);                // above zero, so that a group's largest product is its largest score
+    a8_queries(x, row, e, A.scale_log2 < 0.f, qf);
   }
 
-  // this thread's chunks: row tid / CH + i 256 / CH of the tile
-  const int cr = tid / CH, cc = tid % CH;
-  // Codes are asked for a tile ahead and their pages' numbers two, so that no load waits for another one.
-  const int last = max(f.keys - 1, 0);
+  // this thread's chunks: row tid / CH + i 256 / CH of the tile. Codes are asked for a tile ahead and their pages' numbers two, so
+  // that no load waits for another one.
+  const int cr = tid / CH, cc = tid % CH, last = max(f.keys - 1, 0), mask = (1 << A.sh) - 1;
+  const unsigned page_bytes = ((unsigned)A.G << A.sh) * D;
+  const unsigned char* kat = A.k + ((size_t)kvh << A.sh) * D + cc * 16;
+  const long long to_v = A.v - A.k;
   uint4 kw[N], vw[N];
   int pages[N], group_page = 0;
   float sk = 0.f, sv = 0.f;
   bool there = false;
-  auto look = [&](int tile) {
-    const int kt = tile * A8P_KEYS;
+  auto look = [&](int kt) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) pages[i] = bt[min(kt + cr + i * (256 / CH), last) >> A.sh];
-    group_page = bt[min(kt + 16 * (tid & 3), last) >> A.sh];
+    for (int i = 0; i < N; ++i) pages[i] = bt[(unsigned)min(kt + cr + i * (256 / CH), last) >> A.sh];
+    group_page = bt[(unsigned)min(kt + 16 * (tid & 3), last) >> A.sh];
   };
-  auto fetch = [&](int tile) {
-    const int kt = tile * A8P_KEYS;
+  auto fetch = [&](int kt) __attribute__((always_inline)) {
+    bool none = kt + A8P_KEYS > last + 1;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int key = min(kt + cr + i * (256 / CH), last);
-      const bool ok = (unsigned)pages[i] < (unsigned)A.n_blocks;
-      const size_t off = ((((size_t)(ok ? pages[i] : 0) * A.G + kvh) << A.sh) + (key & ((1 << A.sh) - 1))) * D + cc * 16;
-      kw[i] = *reinterpret_cast<const uint4*>(A.k + off);
-      vw[i] = *reinterpret_cast<const uint4*>(A.v + off);
-      if (__any(!ok || kt + cr + i * (256 / CH) > last)) {   // codes that are none may be NaN, which no weight of zero hides
-        if (!ok || kt + cr + i * (256 / CH) > last) kw[i] = vw[i] = make_uint4(0, 0, 0, 0);
-      }
+      const unsigned key = min(kt + cr + i * (256 / CH), last), page = (unsigned)pages[i] < (unsigned)A.n_blocks ? pages[i] : 0;
+      const unsigned char* at = kat + ((unsigned long long)page * page_bytes + (unsigned)(key & mask) * D);
+      kw[i] = *reinterpret_cast<const uint4*>(at);
+      vw[i] = *reinterpret_cast<const uint4*>(at + to_v);
+      none |= page != (unsigned)pages[i];
+    }
+    if (__any(none)) {                                       // codes that are none may be NaN, which no weight of zero hides
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if ((unsigned)pages[i] >= (unsigned)A.n_blocks || kt + cr + i * (256 / CH) > last) kw[i] = vw[i] = make_uint4(0, 0, 0, 0);
     }
     if (tid < 4) {                                           // the scales of 16 keys
       there = (unsigned)group_page < (unsigned)A.n_blocks;
@@ -469,24 +475,29 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
       sv = A.vs[at];
     }
   };
-  auto store = [&](int stage) {
-    const unsigned at = base + stage * L::STAGE;
+  // piece q of the tile in registers: 8 codes, of keys or of values, widened and put where the fragments are read from
+  // (lanes of a row's upper half put their second part first: eight lanes then write to eight different 16-byte banks)
+  constexpr int PIECES = 4 * N;
+  const bool upper = cc * 2 >= CH;
+  unsigned put_at[4];                                        // K's and V's two parts in the first stage; rows further on keep the swizzle
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int row = cr + i * (256 / CH);
-      const unsigned kr = at + row * (D * 2), vr = kr + L::K;
-      const int ksw = fl_kswz<D>(row), vsw = fl_vswz<D>(row);
-      *fl_lds<c8_h8>(kr + ((2 * cc) ^ ksw) * 16) = c8_widen8<KIND>(kw[i].x, kw[i].y);
-      *fl_lds<c8_h8>(kr + ((2 * cc + 1) ^ ksw) * 16) = c8_widen8<KIND>(kw[i].z, kw[i].w);
-      *fl_lds<c8_h8>(vr + ((2 * cc) ^ vsw) * 16) = c8_widen8<KIND>(vw[i].x, vw[i].y);
-      *fl_lds<c8_h8>(vr + ((2 * cc + 1) ^ vsw) * 16) = c8_widen8<KIND>(vw[i].z, vw[i].w);
-    }
+  for (int q = 0; q < 4; ++q) {
+    const int sw = q & 2 ? fl_vswz<D>(cr) : fl_kswz<D>(cr);
+    put_at[q] = base + (q & 2 ? L::K : 0) + cr * (D * 2) + ((2 * cc + ((q & 1) ^ (int)upper)) ^ sw) * 16;
+  }
+  auto store = [&](int q) __attribute__((always_inline)) {
+    const uint4 w = q & 2 ? vw[q >> 2] : kw[q >> 2];
+    const bool second = (q & 1) != (int)upper;
+    *fl_lds<c8_h8>(put_at[q & 3] + (q >> 2) * (256 / CH) * D * 2) = c8_widen8<KIND>(second ? w.z : w.x, second ? w.w : w.y);
+  };
+  static_assert(256 / CH % 16 == 0, "a thread's rows share a swizzle");
+  auto store_scales = [&](int stage) __attribute__((always_inline)) {
     if (tid < 4) {
       float* s = reinterpret_cast<float*>(lds + L::SCALES + stage * 64) + tid;
       const float vs = a8_least(sv);
       s[0] = there ? a8_least(sk) : 1.f;
       s[4] = there ? __builtin_amdgcn_logf(vs) : -INFINITY;
-      s[8] = there ? 1.f / vs : 0.f;
+      s[8] = there ? __builtin_amdgcn_rcpf(vs) : 0.f;        // off by 2^-23
     }
   };
 
@@ -503,26 +514,43 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   for (int d = 0; d < NDT; ++d) acc[d] = zero;
   float m = A8_NONE, l = 0.f;
   if (n > 0) {
-    look(i0);
-    fetch(i0);
-    look(i0 + 1);
-    store(0);
+    const int kt = i0 * A8P_KEYS;
+    look(kt);
+    fetch(kt);
+    look(kt + A8P_KEYS);
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) store(q);
+    store_scales(0);
+    fetch(kt + A8P_KEYS);
+    look(kt + 2 * A8P_KEYS);
   }
+  constexpr int KR = 4, VR = 4;                              // fragments in flight + 1
+  // rows of this wave that some key of a tile from here on is hidden from, or that end in it
+  const int edge = min(f.keys, A.causal ? f.past + (r0 + wave * 32) / Gq + 1 : f.keys) - A8P_KEYS;
   for (int i = 0; i < n; ++i) {
     const int stage = i & 1, kt = (i0 + i) * A8P_KEYS;
-    if (i + 1 < n) {
-      fetch(i0 + i + 1);
-      look(i0 + i + 2);
-    }
-    __syncthreads();                                         // this stage is written; nobody reads the other one any more
-    float16v s[2] = {zero, zero};
 #pragma unroll
-    for (int u = 0; u < NS; ++u)
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*fl_lds<c8_h8>(kb[u] + stage * L::STAGE + 32 * t * D * 2), qf[u], s[t], 0, 0, 0);
+    for (int q = 0; q < 4; ++q) put_at[q] ^= L::STAGE;       // the other stage
+    fl_meet();                                               // this stage is written, nobody reads the other one any more; loads stay under way
     const float* sc = reinterpret_cast<const float*>(lds + L::SCALES + stage * 64);
-    if (kt + A8P_KEYS > f.keys || (A.causal && kt + A8P_KEYS - 1 > f.past + (r0 + wave * 32) / Gq)) {
+    float16v s[2];
+    c8_h8 kf[KR];
+    auto kread = [&](int u) __attribute__((always_inline)) { kf[u % KR] = *fl_lds<c8_h8>(kb[u >> 1] + 32 * (u & 1) * D * 2); };
+#pragma unroll
+    for (int u = 0; u < KR - 1; ++u) kread(u);
+    // the next tile is widened between the MFMAs of this one's scores
+#pragma unroll
+    for (int u = 0; u < 2 * NS; ++u) {
+      s[u & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[u % KR], qf[u >> 1], u < 2 ? zero : s[u & 1], 0, 0, 0);
+      if (u + KR - 1 < 2 * NS) kread(u + KR - 1);
+      if (u % 2) store(u / 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    static_assert(PIECES == NS, "a piece every other MFMA");
+    store_scales(1 - stage);
+    fetch(kt + 2 * A8P_KEYS);
+    look(kt + 3 * A8P_KEYS);
+    if (kt > edge) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -532,20 +560,22 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
         }
     }
     // t = x c + log2 vs with c above zero: the largest product of a group of 16 keys is its largest score
-    float c[4], lv[4], mx = -INFINITY;
+    const float4v ks = *reinterpret_cast<const float4v*>(sc), lv = *reinterpret_cast<const float4v*>(sc + 4), inv = *reinterpret_cast<const float4v*>(sc + 8);
+    float c[4], mx = -INFINITY;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float k = factor * sc[g];
+      const float k = factor * ks[g];
       c[g] = k < 1.1754943508222875e-38f ? 1.1754943508222875e-38f : k;     // of no use to a masked -infinity if zero; NaN stays
-      lv[g] = sc[4 + g];
       float x = s[g >> 1][8 * (g & 1)];
 #pragma unroll
       for (int j = 1; j < 8; ++j) x = fmaxf(x, s[g >> 1][8 * (g & 1) + j]);
       mx = fmaxf(mx, fmaf(x, c[g], lv[g]));
     }
-    const float m_new = fmaxf(m, fl_max32(mx));
-    if (__any(m_new > m)) {
-      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+    // the reference stays where it is while no row's maximum passes it by more than a factor of 2^8: f16 weights keep their 11
+    // bits up to 2^15, and a prompt's first tiles nearly always raise some row of the wave
+    mx = fl_max32(mx);
+    if (__any(mx > m + 8.f)) {
+      const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
       l *= alpha;
 #pragma unroll
@@ -553,76 +583,129 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[d][j] *= alpha;
     }
+    // the weights of a group of keys between the MFMAs of the group before
+    c8_h8 p[2], vf[VR];
+    auto vread = [&](int v) __attribute__((always_inline)) {
+      const unsigned a = vb[v % NDT] + 16 * (v / NDT) * D * 2;
+      const fl_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a));
+      const fl_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a + 8 * D * 2));
+      short8 a8;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      c8_h8 p;
-      float sum = 0.f;
+      for (int j = 0; j < 4; ++j) { a8[j] = lo[j]; a8[4 + j] = hi[j]; }
+      vf[v % VR] = __builtin_bit_cast(c8_h8, a8);
+    };
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    auto weights = [&](int g, int j0, int j1) __attribute__((always_inline)) {
       const float off = lv[g] - m;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j], c[g], off));
-        sum += e;
-        p[j] = (_Float16)e;
+      for (int j = j0; j < j1; j += 2) {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        const f2 e = {__builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j], c[g], off)),
+                      __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j + 1], c[g], off))};
+        const c8_h2 w = __builtin_convertvector(e, c8_h2);
+        sum[g] += e[0] + e[1];                               // in f32: a weight that f16 has as zero still counts for a page of small values
+        p[g & 1][j] = w[0];
+        p[g & 1][j + 1] = w[1];
       }
-      l = fmaf(sum, sc[8 + g], l);
+    };
 #pragma unroll
-      for (int d = 0; d < NDT; ++d) {
-        const unsigned a = vb[d] + stage * L::STAGE + 16 * g * D * 2;
-        const fl_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a));
-        const fl_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a + 8 * D * 2));
-        short8 a8;
+    for (int v = 0; v < VR - 1; ++v) vread(v);
+    weights(0, 0, 8);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { a8[j] = lo[j]; a8[4 + j] = hi[j]; }
-        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(c8_h8, a8), p, acc[d], 0, 0, 0);
-      }
+    for (int v = 0; v < 4 * NDT; ++v) {
+      const int g = v / NDT, d = v % NDT;
+      acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[v % VR], p[g & 1], acc[d], 0, 0, 0);
+      if (v + VR - 1 < 4 * NDT) vread(v + VR - 1);
+      if (g < 3) weights(g + 1, d * 8 / NDT, (d + 1) * 8 / NDT);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (i + 1 < n) store(1 - stage);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) l = fmaf(sum[g], inv[g], l);
+#pragma unroll
+    for (int u = 0; u < NS; ++u) kb[u] ^= L::STAGE;
+#pragma unroll
+    for (int d = 0; d < NDT; ++d) vb[d] ^= L::STAGE;
   }
   l = fl_both32(l);                                          // a lane has summed up its half of the keys
   const size_t unit = ((size_t)b * A.G + kvh) * A.row_blocks + block;
   const bool whole = (((size_t)A.out | (size_t)A.ldo * 2) & 7) == 0;
-  auto put = [&](int row, int c, const float4v& o, float ls) {
-    const int t = (r0 + row) / Gq;
-    a8_put(A.out + (size_t)(f.q0 + t) * A.ldo + (size_t)(kvh * Gq + r0 + row - t * Gq) * D + c, o, ls, whole);
-  };
   const int row = wave * 32 + (lane & 31);
-  const auto rs = a8_rsrc(A, nparts > 1 ? unit : 0, nparts > 1 ? part : 0, A8P_ROWS, D);
-  if (row < rows) {
+  // Parts of a block's keys: each leaves its accumulators as they lie (16 bytes a lane, a kilobyte a wave), and the last to arrive
+  // adds up all of them, in order, its own from its registers.
+  if (nparts > 1) {
+    constexpr int PER = 256 * (NDT * 16 + 2) * 4;
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc(A.ws + unit * A.parts * (PER / 4), 0, A.parts * PER, 0x00020000);
+    const int at = part * PER + tid * 16, ml = 256 * NDT * 16 * 4 + tid * 8;
 #pragma unroll
-    for (int d = 0; d < NDT; ++d)
+    for (int u = 0; u < 4 * NDT; ++u) {
+      const float4v o = {acc[u / 4][u % 4 * 4], acc[u / 4][u % 4 * 4 + 1], acc[u / 4][u % 4 * 4 + 2], acc[u / 4][u % 4 * 4 + 3]};
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(a8_u4, o), rs, at + u * 4096, 0, 16);
+    }
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(a8_u2, make_float2(m, l)), rs, part * PER + ml, 0, 16);
+    if (!a8_last(A.tickets + unit * TICKET, nparts, reinterpret_cast<int*>(lds))) return;
+    float top = A8_NONE, all = 0.f;
+    for (int p = 0; p < nparts; ++p) top = fmaxf(top, __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, p * PER + ml, 0, 16)).x);
+    float16v total[NDT];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {                          // accumulators 4 u ..: columns 32 d + 8 u + 4 h ..
-        const float4v o = {acc[d][4 * u], acc[d][4 * u + 1], acc[d][4 * u + 2], acc[d][4 * u + 3]};
-        const int c = 32 * d + 8 * u + 4 * h;
-        if (nparts == 1) put(row, c, o, l);
-        else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(a8_u4, o), rs, (row * D + c) * 4, 0, 16);
+    for (int d = 0; d < NDT; ++d) total[d] = zero;
+    for (int p = 0; p < nparts; ++p) {
+      const float2 w = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, p * PER + ml, 0, 16));
+      float4v v[4 * NDT];
+      if (p != part) {
+#pragma unroll
+        for (int u = 0; u < 4 * NDT; ++u) v[u] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(rs, p * PER + tid * 16 + u * 4096, 0, 16));
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4 * NDT; ++u) v[u] = float4v{acc[u / 4][u % 4 * 4], acc[u / 4][u % 4 * 4 + 1], acc[u / 4][u % 4 * 4 + 2], acc[u / 4][u % 4 * 4 + 3]};
       }
-    if (nparts > 1 && h == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(a8_u2, make_float2(m, l)), rs, (A8P_ROWS * D + 2 * row) * 4, 0, 16);
+      const float x = __builtin_amdgcn_exp2f(w.x - top);
+      all = fmaf(x, w.y, all);
+#pragma unroll
+      for (int u = 0; u < 4 * NDT; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) total[u / 4][u % 4 * 4 + j] = fmaf(x, v[u][j], total[u / 4][u % 4 * 4 + j]);
+    }
+    l = all;
+#pragma unroll
+    for (int d = 0; d < NDT; ++d) acc[d] = total[d];
   }
-  if (nparts == 1) return;
-  if (!a8_last(A.tickets + unit * TICKET, nparts, reinterpret_cast<int*>(lds))) return;
-  a8_join<D, A8P_ROWS, 256>(A, unit, nparts, rows, put);
+  if (row < rows) {
+    const int t = (r0 + row) / Gq;
+    bf16_t* at = A.out + (size_t)(f.q0 + t) * A.ldo + (size_t)(kvh * Gq + r0 + row - t * Gq) * D + 4 * h;
+    const float by = l == 0.f ? 0.f : 1.f / l;               // NaN stays
+#pragma unroll
+    for (int u = 0; u < 4 * NDT; ++u) {                      // accumulators 4 u ..: columns 8 u + 4 h ..
+      const uint2 w = make_uint2(pack_bf16x2(acc[u / 4][u % 4 * 4] * by, acc[u / 4][u % 4 * 4 + 1] * by),
+                                 pack_bf16x2(acc[u / 4][u % 4 * 4 + 2] * by, acc[u / 4][u % 4 * 4 + 3] * by));
+      if (whole) {
+        *reinterpret_cast<uint2*>(at + 8 * u) = w;
+      } else {
+        at[8 * u] = (bf16_t)w.x; at[8 * u + 1] = (bf16_t)(w.x >> 16); at[8 * u + 2] = (bf16_t)w.y; at[8 * u + 3] = (bf16_t)(w.y >> 16);
+      }
+    }
+  }
 }
 
-// rows of a workgroup of the form that takes a call: 16 (tokens) or 128 (prompts)
+// parts: of a sequence's keys at most; each: tiles of 64 keys of a prompt's part (the longer blocks have more parts)
 extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const void* v, const void* ks, const void* vs, const void* cu,
                                const void* ctx, const void* bt, void* out, long ldo, int T, int B, int H, int G, int D, int blk, int n_blocks,
-                               int max_blocks, int max_q, float scale, int causal, int kind, int parts, void* ws, long ws_floats, void* tickets,
+                               int max_blocks, int max_q, float scale, int causal, int kind, int parts, int each, void* ws, long ws_floats, void* tickets,
                                long n_tickets, hipStream_t st) {
   if (T <= 0 || B <= 0 || max_q <= 0) return 0;
   if ((D != 64 && D != 128) || (kind != C8_INT8 && kind != C8_E4M3) || blk < 16 || (blk & (blk - 1)) || G <= 0 || H <= 0 || H % G ||
-      n_blocks <= 0 || max_blocks <= 0 || parts <= 0)
+      n_blocks <= 0 || max_blocks <= 0 || parts <= 0 || each <= 0)
     return (int)hipErrorInvalidValue;
   const bool token = (long long)max_q * (H / G) <= A8_ROWS;
   const long long blocks = token ? 1 : ((long long)max_q * (H / G) + A8P_ROWS - 1) / A8P_ROWS, units = (long long)B * G * blocks;
-  const int rows = token ? A8_ROWS : A8P_ROWS;
+  const long long per = token ? A8_ROWS * (D + 2) : A8P_ROWS * (D + 4);     // floats of a part
   if (token ? G > 65535 || B > 65535 || parts > 1 << 24 : units * parts > 1 << 30) return (int)hipErrorInvalidValue;
-  if (blocks > 1 << 24 || (long long)parts * rows * (D + 2) * 4 >= 1LL << 31)
+  if ((long long)G * blk * D >= 1LL << 31 || blocks > 1 << 24 || parts * per * 4 >= 1LL << 31)
     return (int)hipErrorInvalidValue;
-  if (parts > 1 && (!ws || !tickets || ws_floats < units * parts * rows * (D + 2) || n_tickets < units)) return (int)hipErrorInvalidValue;
+  if (parts > 1 && (!ws || !tickets || ws_floats < units * parts * per || n_tickets < units)) return (int)hipErrorInvalidValue;
   const Attn8Args a{(const bf16_t*)q, ldq, (const unsigned char*)k, (const unsigned char*)v, (const float*)ks, (const float*)vs, (const int*)cu,
                     (const int*)ctx, (const int*)bt, (bf16_t*)out, ldo, (float*)ws, (int*)tickets, T, B, H, G, __builtin_ctz(blk), n_blocks, max_blocks,
-                    max_q, parts, causal, (int)blocks, units * parts <= 512, scale * 1.4426950408889634f};
+                    max_q, parts, causal, (int)blocks, each, scale * 1.4426950408889634f};
   if (token) {
     const dim3 grid(parts, G, B);
 #define GO(D_, K_) hipLaunchKernelGGL((attn8_token_kernel<D_, K_>), grid, dim3(A8_WAVES * 64), 0, st, a)

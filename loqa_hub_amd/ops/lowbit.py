@@ -19,6 +19,7 @@ keys as masked. A page that gets rows belongs to one sequence; full pages may be
 from __future__ import annotations
 
 import contextlib
+import functools
 import math
 from typing import NamedTuple
 
@@ -31,6 +32,7 @@ from ._lib import check, kernels, ptr, stream_ptr
 CACHE_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 HEAD_DIMS = (64, 128)
 TOKEN_ROWS, PROMPT_ROWS = 16, 128     # rows of a workgroup of the two forms (csrc/kernels/attn_cache8.hip)
+PROMPT_SLOTS = {64: 768, 128: 512}    # workgroups of the second that the chip holds, by head_dim
 
 
 def _need(ok: bool, what: str) -> None:
@@ -171,12 +173,22 @@ def read8(cache: Cache8, cu_k: torch.Tensor, first: torch.Tensor, block_tables: 
     return k, v
 
 
-def attn8_parts(max_q: int, group: int, units: int, keys: int) -> int:
-    """Parts of a sequence's keys for ``units`` (sequence, kv head) pairs with at most ``keys`` keys."""
+@functools.lru_cache(maxsize=4096)
+def attn8_plan(max_q: int, group: int, units: int, keys: int, D: int, causal: bool) -> tuple[int, int, int, int]:
+    """(parts of a sequence's keys at most, tiles of 64 keys of a prompt's part, floats of workspace, tickets) for ``units``
+    (sequence, kv head) pairs of up to ``max_q`` rows, ``group`` heads and ``keys`` keys."""
     if max_q * group <= TOKEN_ROWS:
-        return max(1, min(-(-512 // units), -(-keys // 128), 64))
-    units *= -(-max_q * group // PROMPT_ROWS)
-    return max(1, min(512 // units, -(-keys // 256), 16))
+        parts = max(1, min(-(-512 // units), -(-keys // 128), 64))
+        return (parts, 1, units * parts * TOKEN_ROWS * (D + 2), units) if parts > 1 else (1, 1, 0, 0)
+    # a prompt's blocks see unlike numbers of keys: parts as long as a workgroup's share of all tiles
+    blocks = -(-max_q * group // PROMPT_ROWS)
+    most = -(-keys // 64)
+    tiles = [min(most, -(-(max(keys - max_q, 0) + min(max_q, (b + 1) * PROMPT_ROWS // group + 1)) // 64)) if causal else most for b in range(blocks)]
+    each = max(4, -(-units * sum(tiles) // PROMPT_SLOTS[D]))
+    parts = min(16, -(-most // each))
+    if parts <= 1:
+        return 1, max(most, 1), 0, 0
+    return parts, max(each, -(-most // parts)), units * blocks * parts * PROMPT_ROWS * (D + 4), units * blocks
 
 
 def attention8(q: torch.Tensor, cache: Cache8, cu_q: torch.Tensor, ctx_lens: torch.Tensor, block_tables: torch.Tensor, *, n_heads: int,
@@ -207,19 +219,13 @@ def attention8(q: torch.Tensor, cache: Cache8, cu_q: torch.Tensor, ctx_lens: tor
         return ref.attention8(q, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, causal=causal, scale=scale, out=out)
     keys = max_blocks * cache.block_size if max_k is None else min(max_k, max_blocks * cache.block_size)
     max_q = min(max_q, T)
-    units = B * G
-    parts = attn8_parts(max_q, H // G, units, max(keys, 1))
+    parts, each, floats, tiles = attn8_plan(max_q, H // G, B * G, max(keys, 1), D, causal)
     st = stream_ptr(q)
-    ws = tickets = None
     with _device(q):
-        if parts > 1:
-            rows = TOKEN_ROWS
-            if max_q * (H // G) > TOKEN_ROWS:
-                rows, units = PROMPT_ROWS, units * -(-max_q * (H // G) // PROMPT_ROWS)
-            ws, tickets = _sk_workspace(q.device, st, units * parts * rows * (D + 2), units)
+        ws, tickets = _sk_workspace(q.device, st, floats, tiles) if parts > 1 else (None, None)
         check(kernels().loqa_attention8(
             ptr(q), q.stride(0), ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale), ptr(cu_q), ptr(ctx_lens), ptr(block_tables),
-            ptr(out), out.stride(0), T, B, H, G, D, cache.block_size, cache.n_blocks, max_blocks, max_q, scale, int(causal), cache.kind, parts,
+            ptr(out), out.stride(0), T, B, H, G, D, cache.block_size, cache.n_blocks, max_blocks, max_q, scale, int(causal), cache.kind, parts, each,
             ptr(ws), 0 if ws is None else ws.numel(), ptr(tickets), 0 if tickets is None else tickets.numel(), st), "attention8")
     return out
 
