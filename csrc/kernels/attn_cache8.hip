@@ -24,7 +24,7 @@ struct Attn8Args {
   long long ldo;
   float* ws;                             // partials: [unit][part][rows][D + 2]
   int* tickets;
-  int T, B, H, G, sh, n_blocks, max_blocks, max_q, parts, causal, row_blocks, each;
+  int T, B, H, G, sh, n_blocks, max_blocks, max_q, parts, causal, row_blocks, each, fold;
   float scale_log2;
 };
 
@@ -410,33 +410,27 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   __shared__ __attribute__((aligned(2 * L::STAGE))) unsigned char lds[L::SMEM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, li = lane & 15;
   // (sequence, kv head) from the workgroup's number modulo as many, so that a head's workgroups share an XCD's L2 where these are a
-  // multiple of eight; blocks of rows from the longest down
-  const int b = blockIdx.x / A.G % A.B, kvh = blockIdx.x % A.G, Gq = A.H / A.G;
-  const int rest = blockIdx.x / A.G / A.B, part = rest % A.parts, turn = rest / A.parts;
+  // multiple of eight
+  const int b = blockIdx.x / A.G % A.B, kvh = blockIdx.x % A.G, Gq = A.H / A.G, rank = blockIdx.x / A.G / A.B;
   const A8Feed f = a8_feed(A, b);
-  const int block = A.row_blocks - 1 - turn;
-  const int r0 = block * A8P_ROWS, rows = min(f.n * Gq - r0, A8P_ROWS);
+  // keys that some row of a block sees, in parts of whole tiles
+  auto rows_of = [&](int block) { return min(f.n * Gq - block * A8P_ROWS, A8P_ROWS); };
+  auto tiles_of = [&](int block) {
+    const int seen = A.causal ? min(f.keys, max(f.past + (block * A8P_ROWS + rows_of(block) - 1) / Gq + 1, 0)) : f.keys;
+    return (seen + A8P_KEYS - 1) / A8P_KEYS;
+  };
+  auto parts_of = [&](int tiles) { return min(max((tiles + A.each - 1) / A.each, 1), A.parts); };
+  // blocks from the longest down; but where all of them are on the chip at once, two a compute unit, the second half from
+  // the shortest up, so that a long and a short one share it
+  const int turn = rank / A.parts, part = rank % A.parts;
+  const int block = A.fold && turn >= (A.row_blocks + 1) / 2 ? turn - (A.row_blocks + 1) / 2 : A.row_blocks - 1 - turn;
+  const int r0 = block * A8P_ROWS, rows = rows_of(block);
   if (rows <= 0) return;
-  // keys that some row of the block sees, in parts of whole tiles
-  const int seen = A.causal ? min(f.keys, max(f.past + (r0 + rows - 1) / Gq + 1, 0)) : f.keys;
-  const int tiles = (seen + A8P_KEYS - 1) / A8P_KEYS, nparts = min(max((tiles + A.each - 1) / A.each, 1), A.parts);
+  const int tiles = tiles_of(block), nparts = parts_of(tiles);
   if (part >= nparts) return;
   const int i0 = (int)((long long)tiles * part / nparts), n = (int)((long long)tiles * (part + 1) / nparts) - i0;
   const unsigned base = fl_lds_at(lds);
   const int* bt = A.bt + (size_t)b * A.max_blocks;
-
-  const int r = r0 + wave * 32 + (lane & 31), tok = min(r / Gq, f.n - 1), qpos = A.causal ? f.past + r / Gq : 0x7fffffff;
-  c8_h8 qf[NS];
-  float factor;
-  {
-    const bool row = r < r0 + rows;
-    const bf16_t* qp = A.q + (size_t)(f.q0 + tok) * A.ldq + (size_t)(kvh * Gq + r % Gq) * D + 8 * h;
-    uint4 x[NS];
-    a8_row(A, x, [&](int u) { return qp + 16 * u; });
-    const int e = a8_lift(fl_max32(a8_top(x)));
-    factor = ldexpf(fabsf(A.scale_log2), -e);                // above zero, so that a group's largest product is its largest score
-    a8_queries(x, row, e, A.scale_log2 < 0.f, qf);
-  }
 
   // this thread's chunks: row tid / CH + i 256 / CH of the tile. Codes are asked for a tile ahead and their pages' numbers two, so
   // that no load waits for another one.
@@ -513,9 +507,22 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
 #pragma unroll
   for (int d = 0; d < NDT; ++d) acc[d] = zero;
   float m = A8_NONE, l = 0.f;
+  if (n > 0) look(i0 * A8P_KEYS);
+  const int r = r0 + wave * 32 + (lane & 31), tok = min(r / Gq, f.n - 1), qpos = A.causal ? f.past + r / Gq : 0x7fffffff;
+  c8_h8 qf[NS];
+  float factor;
+  {
+    const bool row = r < r0 + rows;
+    const bf16_t* qp = A.q + (size_t)(f.q0 + tok) * A.ldq + (size_t)(kvh * Gq + r % Gq) * D + 8 * h;
+    uint4 x[NS];
+    a8_row(A, x, [&](int u) { return qp + 16 * u; });
+    const int e = a8_lift(fl_max32(a8_top(x)));
+    factor = ldexpf(fabsf(A.scale_log2), -e);                // above zero, so that a group's largest product is its largest score
+    a8_queries(x, row, e, A.scale_log2 < 0.f, qf);
+  }
+
   if (n > 0) {
     const int kt = i0 * A8P_KEYS;
-    look(kt);
     fetch(kt);
     look(kt + A8P_KEYS);
 #pragma unroll
@@ -705,7 +712,7 @@ extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const voi
   if (parts > 1 && (!ws || !tickets || ws_floats < units * parts * per || n_tickets < units)) return (int)hipErrorInvalidValue;
   const Attn8Args a{(const bf16_t*)q, ldq, (const unsigned char*)k, (const unsigned char*)v, (const float*)ks, (const float*)vs, (const int*)cu,
                     (const int*)ctx, (const int*)bt, (bf16_t*)out, ldo, (float*)ws, (int*)tickets, T, B, H, G, __builtin_ctz(blk), n_blocks, max_blocks,
-                    max_q, parts, causal, (int)blocks, each, scale * 1.4426950408889634f};
+                    max_q, parts, causal, (int)blocks, each, parts == 1 && units <= 512, scale * 1.4426950408889634f};
   if (token) {
     const dim3 grid(parts, G, B);
 #define GO(D_, K_) hipLaunchKernelGGL((attn8_token_kernel<D_, K_>), grid, dim3(A8_WAVES * 64), 0, st, a)

@@ -174,21 +174,15 @@ def read8(cache: Cache8, cu_k: torch.Tensor, first: torch.Tensor, block_tables: 
 
 
 @functools.lru_cache(maxsize=4096)
-def attn8_plan(max_q: int, group: int, units: int, keys: int, D: int, causal: bool) -> tuple[int, int, int, int]:
+def attn8_plan(max_q: int, group: int, units: int, keys: int, D: int) -> tuple[int, int, int, int]:
     """(parts of a sequence's keys at most, tiles of 64 keys of a prompt's part, floats of workspace, tickets) for ``units``
     (sequence, kv head) pairs of up to ``max_q`` rows, ``group`` heads and ``keys`` keys."""
     if max_q * group <= TOKEN_ROWS:
         parts = max(1, min(-(-512 // units), -(-keys // 128), 64))
         return (parts, 1, units * parts * TOKEN_ROWS * (D + 2), units) if parts > 1 else (1, 1, 0, 0)
-    # a prompt's blocks see unlike numbers of keys: parts as long as a workgroup's share of all tiles
-    blocks = -(-max_q * group // PROMPT_ROWS)
-    most = -(-keys // 64)
-    tiles = [min(most, -(-(max(keys - max_q, 0) + min(max_q, (b + 1) * PROMPT_ROWS // group + 1)) // 64)) if causal else most for b in range(blocks)]
-    each = max(4, -(-units * sum(tiles) // PROMPT_SLOTS[D]))
-    parts = min(16, -(-most // each))
-    if parts <= 1:
-        return 1, max(most, 1), 0, 0
-    return parts, max(each, -(-most // parts)), units * blocks * parts * PROMPT_ROWS * (D + 4), units * blocks
+    blocks, most = -(-max_q * group // PROMPT_ROWS), max(1, -(-keys // 64))
+    parts = max(1, min(PROMPT_SLOTS[D] // (units * blocks), most // 4, 16))
+    return (parts, -(-most // parts), units * blocks * parts * PROMPT_ROWS * (D + 4), units * blocks) if parts > 1 else (1, most, 0, 0)
 
 
 def attention8(q: torch.Tensor, cache: Cache8, cu_q: torch.Tensor, ctx_lens: torch.Tensor, block_tables: torch.Tensor, *, n_heads: int,
@@ -219,7 +213,7 @@ def attention8(q: torch.Tensor, cache: Cache8, cu_q: torch.Tensor, ctx_lens: tor
         return ref.attention8(q, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, causal=causal, scale=scale, out=out)
     keys = max_blocks * cache.block_size if max_k is None else min(max_k, max_blocks * cache.block_size)
     max_q = min(max_q, T)
-    parts, each, floats, tiles = attn8_plan(max_q, H // G, B * G, max(keys, 1), D, causal)
+    parts, each, floats, tiles = attn8_plan(max_q, H // G, B * G, max(keys, 1), D)
     st = stream_ptr(q)
     with _device(q):
         ws, tickets = _sk_workspace(q.device, st, floats, tiles) if parts > 1 else (None, None)
