@@ -508,7 +508,7 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   for (int d = 0; d < NDT; ++d) acc[d] = zero;
   float m = A8_NONE, l = 0.f;
   if (n > 0) look(i0 * A8P_KEYS);
-  const int r = r0 + wave * 32 + (lane & 31), tok = min(r / Gq, f.n - 1), qpos = A.causal ? f.past + r / Gq : 0x7fffffff;
+  const int r = r0 + wave * 32 + (lane & 31), tok = min(r / Gq, f.n - 1), seen = min(A.causal ? f.past + r / Gq : 0x7fffffff, f.keys - 1);
   c8_h8 qf[NS];
   float factor;
   {
@@ -563,7 +563,7 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int key = kt + 32 * t + (j & 3) + 8 * (j >> 2) + 4 * h;
-          if (key >= f.keys || key > qpos) s[t][j] = -INFINITY;
+          if (key > seen) s[t][j] = -INFINITY;
         }
     }
     // t = x c + log2 vs with c above zero: the largest product of a group of 16 keys is its largest score

@@ -6,9 +6,10 @@
 // token with the checks before them: 24.5 us through ctypes, 14.4 through this. Latent attention's steps, which are short prompts as
 // well, come through here too.
 //
-// The symbols are libloqa_seqmix.so's, which is loaded before this module; signatures() lets the loader compare the
+// The symbols are libloqa_seqmix.so's and libloqa_lowbit.so's, which are loaded before this module; signatures() lets the loader compare the
 // types here with those it knows.
 #include <Python.h>
+#include <ATen/ops/empty.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <exception>
@@ -45,6 +46,15 @@ int loqa_latent_prefill(const void*, long, const void*, const void*, void*, long
 int loqa_sigmoid_gate(const void*, long, long, int, const void*, long, void*, long, long, int, int, int, stream_t);
 int loqa_head_product(const void*, long, long, const void*, int, int, int, int, void*, long, long, stream_t);
 int loqa_moe_route(const void*, const void*, const void*, int, int, int, int, int, int, int, float, void*, void*, int, stream_t);
+int loqa_rope_append8(const void*, long, const void*, int, void*, void*, void*, void*, const void*, const void*, const void*, void*, long, int,
+                      int, int, int, int, int, int, int, int, int, stream_t);
+int loqa_read8(const void*, const void*, const void*, const void*, const void*, const void*, const void*, void*, void*, int, int, int, int, int,
+               int, int, int, stream_t);
+int loqa_attention8(const void*, long, const void*, const void*, const void*, const void*, const void*, const void*, const void*, void*, long,
+                    int, int, int, int, int, int, int, int, int, float, int, int, int, int, void*, long, void*, long, stream_t);
+int loqa_page_step(const void*, const void*, void*, void*, const void*, void*, void*, void*, void*, void*, void*, void*, void*, int, int, int,
+                   int, int, stream_t);
+int loqa_linear4(const void*, long, const void*, const void*, const void*, const void*, void*, long, int, int, int, int, stream_t);
 }
 
 namespace {
@@ -221,10 +231,75 @@ PyObject* window_shapes(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// ---- ops/lowbit.py. What its checks ask of a call's tensors, in one go: the numbers of the launch and what it writes to, or None where
+// anything is not as a GPU call has it (the checks there then say what, or take the tensors to the CPU's forms).
+bool i32_on(const at::Tensor* t, const at::Device& dev) {
+  return t && t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == dev;
+}
+bool rows_on(const at::Tensor& t, long cols, const at::Device& dev) {
+  return t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.size(1) >= cols && (t.stride(1) == 1 || t.size(1) == 1) &&
+         (t.size(0) <= 1 || t.stride(0) >= cols) && t.device() == dev;
+}
+at::Tensor made(at::IntArrayRef size, at::ScalarType type, const at::Device& dev) {
+  return at::empty(size, at::TensorOptions().dtype(type).device(dev));
+}
+
+// (rows x, rows y or None, cu_q, ctx_lens, block_tables, the cache's k; columns of x, of y) -> (T, B, columns of the
+// table, row strides of x and y, y, device)
+PyObject* cache8_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return checked<6, 2>(args, n, [](const at::Tensor* const* t, const long* v) -> PyObject* {
+    if (!t[0] || !t[5] || !t[5]->is_cuda()) Py_RETURN_NONE;
+    const at::Tensor &x = *t[0], &bt = *t[4];
+    const at::Device dev = t[5]->device();
+    if (!rows_on(x, v[0], dev) || (t[1] && (!rows_on(*t[1], v[1], dev) || t[1]->size(0) != x.size(0)))) Py_RETURN_NONE;
+    if (!i32_on(t[2], dev) || !i32_on(t[3], dev) || !i32_on(t[4], dev)) Py_RETURN_NONE;
+    const long T = x.size(0), B = t[3]->numel();
+    if (T == 0 || B == 0 || t[2]->numel() != B + 1 || bt.dim() != 2 || bt.size(0) != B || bt.size(1) == 0) Py_RETURN_NONE;
+    const at::Tensor y = t[1] ? *t[1] : made({T, v[1]}, at::kBFloat16, dev);
+    return Py_BuildValue("lllllNl", T, B, (long)bt.size(1), (long)x.stride(0), (long)y.stride(0), THPVariable_Wrap(y), (long)dev.index());
+  });
+}
+
+// (new_lens, ctx_lens, block_tables, free_pages, ring, ctx_out or None, ring_out or None; max_tokens) -> (B, columns, pool, cu_q,
+// positions, slots, last_rows, ctx_out, ring_out, status, device)
+PyObject* page_tensors(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return checked<7, 1>(args, n, [](const at::Tensor* const* t, const long* v) -> PyObject* {
+    if (!t[2] || !t[2]->is_cuda()) Py_RETURN_NONE;
+    const at::Device dev = t[2]->device();
+    for (int i = 0; i < 7; ++i)
+      if (i < 5 ? !i32_on(t[i], dev) : t[i] && !i32_on(t[i], dev)) Py_RETURN_NONE;
+    const at::Tensor& bt = *t[2];
+    const long B = t[0]->numel(), pool = t[3]->numel(), most = v[0];
+    if (B == 0 || t[1]->numel() != B || bt.dim() != 2 || bt.size(0) != B || bt.size(1) == 0 || t[4]->numel() != 2 || pool == 0 || most < 0)
+      Py_RETURN_NONE;
+    if ((t[5] && t[5]->numel() != B) || (t[6] && t[6]->numel() != 2)) Py_RETURN_NONE;
+    auto ints = [&](long m) { return THPVariable_Wrap(made({m}, at::kInt, dev)); };
+    return Py_BuildValue("lllNNNNNNNl", B, (long)bt.size(1), pool, ints(B + 1), ints(most), ints(most), THPVariable_Wrap(made({B}, at::kLong, dev)),
+                         t[5] ? THPVariable_Wrap(*t[5]) : ints(B), t[6] ? THPVariable_Wrap(*t[6]) : ints(2), ints(1), (long)dev.index());
+  });
+}
+
+// (x, the weight's codes, bias or None; N, K) -> (rows, row stride, y [rows of x.., N], device)
+PyObject* linear4_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return checked<3, 2>(args, n, [](const at::Tensor* const* t, const long* v) -> PyObject* {
+    if (!t[0] || !t[1] || !t[1]->is_cuda()) Py_RETURN_NONE;
+    const at::Tensor& x = *t[0];
+    const at::Device dev = t[1]->device();
+    const long N = v[0], K = v[1];
+    if (x.scalar_type() != at::kBFloat16 || x.device() != dev || x.dim() != 2 || x.size(1) != K || x.size(0) == 0 || x.stride(1) != 1 ||
+        x.stride(0) < 0 || x.stride(0) % 8 || ((size_t)x.data_ptr() & 15))
+      Py_RETURN_NONE;
+    if (t[2] && (t[2]->scalar_type() != at::kBFloat16 || t[2]->dim() != 1 || t[2]->size(0) != N || !t[2]->is_contiguous() || t[2]->device() != dev))
+      Py_RETURN_NONE;
+    return Py_BuildValue("llNl", (long)x.size(0), (long)x.stride(0), THPVariable_Wrap(made({x.size(0), N}, at::kBFloat16, dev)), (long)dev.index());
+  });
+}
+
 #define ENTRIES(X)                                                                                                                \
   X(loqa_qk_prep_append) X(loqa_window_attention) X(loqa_window_attention_parts) X(loqa_delta_prep) X(loqa_delta_scan) \
   X(loqa_seq_state_save) X(loqa_gated_rmsnorm) X(loqa_moe_route) X(loqa_latent_attention) X(loqa_latent_kv) \
-  X(loqa_latent_prefill) X(loqa_sigmoid_gate) X(loqa_head_product)
+  X(loqa_latent_prefill) X(loqa_sigmoid_gate) X(loqa_head_product) \
+  X(loqa_rope_append8) X(loqa_read8) X(loqa_attention8) X(loqa_page_step) X(loqa_linear4)
 
 PyObject* signatures(PyObject*, PyObject*) {
   PyObject* d = PyDict_New();
@@ -246,6 +321,9 @@ PyMethodDef methods[] = {
     {"f32c", (PyCFunction)(void (*)(void))contiguous<at::kFloat>, METH_FASTCALL, nullptr},
     {"qk_shapes", (PyCFunction)(void (*)(void))qk_shapes, METH_FASTCALL, nullptr},
     {"window_shapes", (PyCFunction)(void (*)(void))window_shapes, METH_FASTCALL, nullptr},
+    {"cache8_rows", (PyCFunction)(void (*)(void))cache8_rows, METH_FASTCALL, nullptr},
+    {"page_tensors", (PyCFunction)(void (*)(void))page_tensors, METH_FASTCALL, nullptr},
+    {"linear4_rows", (PyCFunction)(void (*)(void))linear4_rows, METH_FASTCALL, nullptr},
     {"signatures", signatures, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 #undef METHOD

@@ -350,7 +350,9 @@ def _main_kernels() -> ctypes.CDLL:
 # tensors, addresses or None. i32c and f32c check (tensor, name) pairs, the others the tensors of a launch.
 _LAUNCH = frozenset(("loqa_qk_prep_append", "loqa_window_attention", "loqa_window_attention_parts", "loqa_delta_prep",
                      "loqa_delta_scan", "loqa_seq_state_save", "loqa_gated_rmsnorm", "loqa_moe_route", "loqa_latent_attention",
-                     "loqa_latent_kv", "loqa_latent_prefill", "loqa_sigmoid_gate", "loqa_head_product", "i32c", "f32c", "qk_shapes", "window_shapes"))
+                     "loqa_latent_kv", "loqa_latent_prefill", "loqa_sigmoid_gate", "loqa_head_product", "i32c", "f32c", "qk_shapes", "window_shapes",
+                     "loqa_rope_append8", "loqa_read8", "loqa_attention8", "loqa_page_step", "loqa_linear4", "cache8_rows", "page_tensors",
+                     "linear4_rows"))
 _launch = None
 
 
@@ -359,6 +361,7 @@ def launch():
     global _launch
     if _launch is None:
         seqmix()                                  # its symbols
+        lowbit()
         with _lock:
             if _launch is None:
                 path = os.path.join(_NATIVE, "libloqa_launch.so")
@@ -368,8 +371,9 @@ def launch():
                 mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("libloqa_launch", loader))
                 loader.exec_module(mod)
                 code = {_vp: "p", _i: "i", _l: "l", _f: "f"}
+                known = {**_SEQMIX_SIGS, **_LOWBIT_SIGS}
                 for fn, sig in mod.signatures().items():
-                    if sig != "".join(code[t] for t in _SEQMIX_SIGS[fn]):
+                    if sig != "".join(code[t] for t in known[fn]):
                         raise RuntimeError(f"{fn}: libloqa_launch.so was built for other arguments")
                 _launch = mod
     return _launch

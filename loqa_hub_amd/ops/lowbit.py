@@ -51,9 +51,13 @@ def _i32(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
     _need(t.device == like.device, f"{name} must be on {like.device}")
 
 
-def _device(t: torch.Tensor):
+def _there(index: int):
     """Launches go to the tensors' own device, whichever is the current one."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+_HERE = contextlib.nullcontext()
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
 class Cache8:
@@ -64,7 +68,7 @@ class Cache8:
     once is off by half a step. e4m3 scales are powers of two, whose growth rounds nothing again but the smallest
     entries. Scales below 2^-100 count as 2^-100. Page sizes are powers of two from 16 on."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "kind", "n_blocks", "n_kv", "block_size", "head_dim")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "kind", "n_blocks", "n_kv", "block_size", "head_dim", "cuda")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dtype not in CACHE_TYPES:
@@ -77,7 +81,7 @@ class Cache8:
         _need(all(t.is_contiguous() and t.device == k.device for t in (k, v, k_scale, v_scale)), "contiguous tensors of one device")
         _need((k.data_ptr() | v.data_ptr()) % 16 == 0, "k and v must start at 16 bytes")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.kind = CACHE_TYPES[k.dtype]
+        self.kind, self.cuda = CACHE_TYPES[k.dtype], k.is_cuda
         self.n_blocks, self.n_kv, self.block_size, self.head_dim = k.shape
         _need(self.n_blocks > 0 and self.n_kv > 0, "a cache without pages")
         _need(self.head_dim in HEAD_DIMS, f"head_dim is one of {HEAD_DIMS}, got {self.head_dim}")
@@ -117,6 +121,11 @@ def _rows(t: torch.Tensor, cols: int, name: str, like) -> None:
     _need(t.device == like.device, f"{name} must be on {like.device}")
 
 
+def _rows8(x, y, cu_q, ctx_lens, block_tables, cache, cols: int, cols_y: int):
+    """All of a GPU call's checks of its rows and sequences at once (csrc/launch); None: anything is otherwise."""
+    return kernels().cache8_rows(x, y, cu_q, ctx_lens, block_tables, cache.k, cols, cols_y) if cache.cuda else None
+
+
 def rope_append8(qkv: torch.Tensor, cos_sin: torch.Tensor | None, cache: Cache8, cu_q: torch.Tensor, ctx_lens: torch.Tensor,
                  block_tables: torch.Tensor, *, n_heads: int, max_q: int, q_out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotate q and k of a step and append k / v to the cache; returns the rotated queries [T, H * D] bf16 (``q_out``
@@ -128,28 +137,30 @@ def rope_append8(qkv: torch.Tensor, cos_sin: torch.Tensor | None, cache: Cache8,
     appended. An infinite or NaN entry makes its page's scale so, and with it what attention gives for the page."""
     H, G, D = n_heads, cache.n_kv, cache.head_dim
     _need(H > 0 and max_q >= 0, "n_heads and max_q")
-    _rows(qkv, (H + 2 * G) * D, "qkv", cache)
-    T = qkv.shape[0]
-    B, max_blocks = _sequences(cu_q, ctx_lens, block_tables, cache)
     if cos_sin is not None:
         _typed(cos_sin, torch.float32, "cos_sin")
         _need(cos_sin.dim() == 3 and cos_sin.shape[1:] == (D // 2, 2) and cos_sin.shape[0] > 0 and cos_sin.is_contiguous()
               and cos_sin.device == cache.device and cos_sin.data_ptr() % 16 == 0, "cos_sin is [max_pos, head_dim / 2, 2], contiguous")
-    if q_out is None:
-        q_out = torch.empty(T, H * D, dtype=torch.bfloat16, device=qkv.device)
-    else:
+    fast = _rows8(qkv, q_out, cu_q, ctx_lens, block_tables, cache, (H + 2 * G) * D, H * D)
+    if fast is None:
+        _rows(qkv, (H + 2 * G) * D, "qkv", cache)
+        T = qkv.shape[0]
+        B, _ = _sequences(cu_q, ctx_lens, block_tables, cache)
+        if q_out is None:
+            q_out = torch.empty(T, H * D, dtype=torch.bfloat16, device=qkv.device)
         _rows(q_out, H * D, "q_out", cache)
         _need(q_out.shape[0] == T, "q_out has the rows of qkv")
-    if T == 0 or B == 0 or max_q == 0:
+        return q_out if T == 0 or B == 0 or max_q == 0 else \
+            ref.rope_append8(qkv, cos_sin, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, q_out=q_out)
+    T, B, max_blocks, ld, ldq, q_out, dev = fast
+    if max_q == 0:
         return q_out
-    if not qkv.is_cuda:
-        return ref.rope_append8(qkv, cos_sin, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, q_out=q_out)
-    _need((qkv.data_ptr() | q_out.data_ptr()) % 8 == 0 and (qkv.stride(0) | q_out.stride(0)) % 4 == 0, "rows of qkv and q_out must start at 8 bytes")
-    with _device(qkv):
+    _need((qkv.data_ptr() | q_out.data_ptr()) % 8 == 0 and (ld | ldq) % 4 == 0, "rows of qkv and q_out must start at 8 bytes")
+    with _there(dev):
         check(kernels().loqa_rope_append8(
-            ptr(qkv), qkv.stride(0), ptr(cos_sin), 0 if cos_sin is None else cos_sin.shape[0], ptr(cache.k), ptr(cache.v), ptr(cache.k_scale),
-            ptr(cache.v_scale), ptr(cu_q), ptr(ctx_lens), ptr(block_tables), ptr(q_out), q_out.stride(0), T, B, H, G, D, cache.block_size,
-            cache.n_blocks, max_blocks, min(max_q, T), cache.kind, stream_ptr(qkv)), "rope_append8")
+            qkv, ld, cos_sin, 0 if cos_sin is None else cos_sin.shape[0], cache.k, cache.v, cache.k_scale, cache.v_scale, cu_q, ctx_lens,
+            block_tables, q_out, ldq, T, B, H, G, D, cache.block_size, cache.n_blocks, max_blocks, min(max_q, T), cache.kind, _stream(dev)),
+            "rope_append8")
     return q_out
 
 
@@ -159,17 +170,17 @@ def read8(cache: Cache8, cu_k: torch.Tensor, first: torch.Tensor, block_tables: 
     rows of no sequence are zeros too."""
     B, max_blocks = _sequences(cu_k, first, block_tables, cache)
     _need(0 <= total < 1 << 31, "total")
-    k, v = (torch.empty(total, cache.n_kv, cache.head_dim, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
-    if not cache.k.is_cuda:
+    shape = (total, cache.n_kv, cache.head_dim)
+    k = torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device)
+    v = torch.empty_like(k)
+    if not cache.cuda:
         return ref.read8(cache, cu_k, first, block_tables, k.zero_(), v.zero_())
-    if total == 0:
-        return k, v
-    if B == 0:
+    if total == 0 or B == 0:
         return k.zero_(), v.zero_()
-    with _device(k):
-        check(kernels().loqa_read8(ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale), ptr(cu_k), ptr(first), ptr(block_tables),
-                                   ptr(k), ptr(v), total, B, cache.n_kv, cache.head_dim, cache.block_size, cache.n_blocks, max_blocks,
-                                   cache.kind, stream_ptr(k)), "read8")
+    dev = k.get_device()
+    with _there(dev):
+        check(kernels().loqa_read8(cache.k, cache.v, cache.k_scale, cache.v_scale, cu_k, first, block_tables, k, v, total, B, cache.n_kv,
+                                   cache.head_dim, cache.block_size, cache.n_blocks, max_blocks, cache.kind, _stream(dev)), "read8")
     return k, v
 
 
@@ -198,29 +209,31 @@ def attention8(q: torch.Tensor, cache: Cache8, cu_q: torch.Tensor, ctx_lens: tor
     H, G, D = n_heads, cache.n_kv, cache.head_dim
     _need(H > 0 and H % G == 0, "n_heads must be a multiple of the cache's heads")
     _need(max_q >= 0 and (max_k is None or max_k >= 0), "max_q and max_k")
-    _rows(q, H * D, "q", cache)
-    T = q.shape[0]
-    B, max_blocks = _sequences(cu_q, ctx_lens, block_tables, cache)
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if out is None:
-        out = torch.empty(T, H * D, dtype=torch.bfloat16, device=q.device)
-    else:
+    scale = D ** -0.5 if scale is None else float(scale)
+    fast = _rows8(q, out, cu_q, ctx_lens, block_tables, cache, H * D, H * D)
+    if fast is None:
+        _rows(q, H * D, "q", cache)
+        T = q.shape[0]
+        B, _ = _sequences(cu_q, ctx_lens, block_tables, cache)
+        if out is None:
+            out = torch.empty(T, H * D, dtype=torch.bfloat16, device=q.device)
         _rows(out, H * D, "out", cache)
         _need(out.shape[0] == T, "out has the rows of q")
-    if T == 0 or B == 0 or max_q == 0:
+        return out if T == 0 or B == 0 or max_q == 0 else \
+            ref.attention8(q, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, causal=causal, scale=scale, out=out)
+    T, B, max_blocks, ldq, ldo, out, dev = fast
+    if max_q == 0:
         return out
-    if not q.is_cuda:
-        return ref.attention8(q, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, causal=causal, scale=scale, out=out)
     keys = max_blocks * cache.block_size if max_k is None else min(max_k, max_blocks * cache.block_size)
     max_q = min(max_q, T)
     parts, each, floats, tiles = attn8_plan(max_q, H // G, B * G, max(keys, 1), D)
-    st = stream_ptr(q)
-    with _device(q):
+    st = _stream(dev)
+    with _there(dev):
         ws, tickets = _sk_workspace(q.device, st, floats, tiles) if parts > 1 else (None, None)
         check(kernels().loqa_attention8(
-            ptr(q), q.stride(0), ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale), ptr(cu_q), ptr(ctx_lens), ptr(block_tables),
-            ptr(out), out.stride(0), T, B, H, G, D, cache.block_size, cache.n_blocks, max_blocks, max_q, scale, int(causal), cache.kind, parts, each,
-            ptr(ws), 0 if ws is None else ws.numel(), ptr(tickets), 0 if tickets is None else tickets.numel(), st), "attention8")
+            q, ldq, cache.k, cache.v, cache.k_scale, cache.v_scale, cu_q, ctx_lens, block_tables, out, ldo, T, B, H, G, D, cache.block_size,
+            cache.n_blocks, max_blocks, max_q, scale, int(causal), cache.kind, parts, each, ws, 0 if ws is None else ws.numel(), tickets,
+            0 if tickets is None else tickets.numel(), st), "attention8")
     return out
 
 
@@ -253,35 +266,36 @@ def page_step(new_lens: torch.Tensor, ctx_lens: torch.Tensor, block_tables: torc
     sequences and given back behind the last free one. ``ctx_out`` / ``ring_out`` may be ``ctx_lens`` / ``ring`` themselves.
     All or nothing: where the status is not 0, nothing changes and no token has a slot. At most 4096 sequences. A page that
     several sequences share must not be given back here."""
-    _typed(block_tables, torch.int32, "block_tables")
-    for t, name in ((new_lens, "new_lens"), (ctx_lens, "ctx_lens"), (block_tables, "block_tables"), (free_pages, "free_pages"), (ring, "ring")):
-        _i32(t, name, block_tables)
-    B, pool = new_lens.numel(), free_pages.numel()
-    _need(0 < B <= PAGE_STEP_SEQS, f"1 to {PAGE_STEP_SEQS} sequences")
-    _need(ctx_lens.numel() == B and block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.shape[1] > 0, "ctx_lens [B], block_tables [B, max_blocks]")
-    _need(ring.numel() == 2 and pool > 0, "ring [2], free_pages [N]")
-    _need(block_size > 0 and block_size & (block_size - 1) == 0 and pool * block_size < 1 << 31, "block_size is a power of two, slots have 32 bits")
     _need(0 <= max_tokens <= 1 << 30, "max_tokens")
-    dev, i32 = block_tables.device, torch.int32
-    if ctx_out is None:
-        ctx_out = torch.empty(B, dtype=i32, device=dev)
-    if ring_out is None:
-        ring_out = torch.empty(2, dtype=i32, device=dev)
-    for t, n, name in ((ctx_out, B, "ctx_out"), (ring_out, 2, "ring_out")):
-        _i32(t, name, block_tables)
-        _need(t.numel() == n, f"{name} has {n} entries")
-    step = PageStep(torch.empty(B + 1, dtype=i32, device=dev), torch.empty(max_tokens, dtype=i32, device=dev),
-                    torch.empty(max_tokens, dtype=i32, device=dev), torch.empty(B, dtype=torch.int64, device=dev), ctx_out, ring_out,
-                    torch.empty(1, dtype=i32, device=dev))
-    if not block_tables.is_cuda:
+    fast = kernels().page_tensors(new_lens, ctx_lens, block_tables, free_pages, ring, ctx_out, ring_out, max_tokens) if block_tables.is_cuda else None
+    if fast is None:
+        _typed(block_tables, torch.int32, "block_tables")
+        for t, name in ((new_lens, "new_lens"), (ctx_lens, "ctx_lens"), (block_tables, "block_tables"), (free_pages, "free_pages"), (ring, "ring"),
+                        (ctx_out, "ctx_out"), (ring_out, "ring_out")):
+            if t is not None:
+                _i32(t, name, block_tables)
+        B, pool = new_lens.numel(), free_pages.numel()
+        _need(B > 0, "no sequences")
+        _need(ctx_lens.numel() == B and block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.shape[1] > 0, "ctx_lens [B], block_tables [B, max_blocks]")
+        _need(ring.numel() == 2 and pool > 0, "ring [2], free_pages [N]")
+        for t, n, name in ((ctx_out, B, "ctx_out"), (ring_out, 2, "ring_out")):
+            _need(t is None or t.numel() == n, f"{name} has {n} entries")
+    else:
+        B, width, pool = fast[:3]
+    _need(B <= PAGE_STEP_SEQS, f"at most {PAGE_STEP_SEQS} sequences")
+    _need(block_size > 0 and block_size & (block_size - 1) == 0 and pool * block_size < 1 << 31, "block_size is a power of two, slots have 32 bits")
+    if fast is None:
+        def ints(n, dtype=torch.int32):
+            return torch.empty(n, dtype=dtype, device=block_tables.device)
+        step = PageStep(ints(B + 1), ints(max_tokens), ints(max_tokens), ints(B, torch.int64), ints(B) if ctx_out is None else ctx_out,
+                        ints(2) if ring_out is None else ring_out, ints(1))
         return ref.page_step(new_lens, ctx_lens, block_tables, free_pages, ring, block_size, step)
-    st = stream_ptr(block_tables)
-    with _device(block_tables):
-        _, tickets = _sk_workspace(dev, st, 1, 1)
-        check(kernels().loqa_page_step(
-            ptr(new_lens), ptr(ctx_lens), ptr(block_tables), ptr(free_pages), ptr(ring), ptr(step.cu_q), ptr(step.positions), ptr(step.slots),
-            ptr(step.last_rows), ptr(ctx_out), ptr(ring_out), ptr(step.status), ptr(tickets), B, block_tables.shape[1], block_size, pool,
-            max_tokens, st), "page_step")
+    step, dev = PageStep._make(fast[3:10]), fast[10]
+    st = _stream(dev)
+    with _there(dev):
+        _, tickets = _sk_workspace(block_tables.device, st, 1, 1)
+        check(kernels().loqa_page_step(new_lens, ctx_lens, block_tables, free_pages, ring, step.cu_q, step.positions, step.slots, step.last_rows,
+                                       step.ctx_lens, step.ring, step.status, tickets, B, width, block_size, pool, max_tokens, st), "page_step")
     return step
 
 
@@ -325,7 +339,7 @@ class Weight4:
             _typed(zeros, torch.uint8, "zeros")
             _need(zeros.shape == scales.shape, "zeros have the shape of scales")
         _need(all(t is None or t.device == codes.device for t in (scales, zeros)), "tensors of one device")
-        self.device = codes.device
+        self.cuda = codes.is_cuda
         codes, scales = codes.contiguous(), scales.contiguous()
         zeros = None if zeros is None else zeros.contiguous()
         if not codes.is_cuda:
@@ -335,7 +349,7 @@ class Weight4:
         self.codes = torch.empty(tiles * blocks * 256, dtype=torch.int32, device=codes.device)
         self.scales = torch.empty(tiles * groups * 16, dtype=torch.bfloat16, device=codes.device)
         self.zeros = None if zeros is None else torch.empty(tiles * groups * 16, dtype=torch.uint8, device=codes.device)
-        with _device(codes):
+        with _there(codes.get_device()):
             check(kernels().loqa_shuffle4(ptr(codes), ptr(scales), ptr(zeros), ptr(self.codes), ptr(self.scales), ptr(self.zeros), self.n, self.k,
                                           self.group, stream_ptr(codes)), "shuffle4")
 
@@ -350,22 +364,21 @@ class Weight4:
 def linear4(x: torch.Tensor, w: Weight4, b: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] bf16 times the transpose of a 4-bit weight (+ bias [N] bf16): [..., N] bf16, summed up in f32. Made for
     the few rows of token steps; more than 64 read the weight again for every 64. An infinite or NaN entry of x makes its row NaN."""
-    _typed(x, torch.bfloat16, "x")
-    _need(x.dim() >= 1 and x.shape[-1] == w.k, f"x has {w.k} columns")
-    _need(x.device == w.device, f"x must be on {w.device}")
-    if b is not None:
-        _typed(b, torch.bfloat16, "b")
-        _need(b.shape == (w.n,) and b.is_contiguous() and b.device == w.device, f"b is [{w.n}], contiguous")
-    if not x.is_cuda:
-        return ref.linear4(x, w, b)
-    y = torch.empty(*x.shape[:-1], w.n, dtype=torch.bfloat16, device=x.device)
-    x2 = x if x.dim() == 2 else x.reshape(-1, w.k)
-    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < 0 or x2.data_ptr() % 16:
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    M = x2.shape[0]
-    if M == 0:
-        return y
-    with _device(x):
-        check(kernels().loqa_linear4(ptr(x2), x2.stride(0), ptr(w.codes), ptr(w.scales), ptr(w.zeros), ptr(b), ptr(y), w.n, M, w.n, w.k, w.group,
-                                     stream_ptr(x)), "linear4")
+    fast = kernels().linear4_rows(x, w.codes, b, w.n, w.k) if w.cuda else None
+    if fast is None:
+        _typed(x, torch.bfloat16, "x")
+        _need(x.dim() >= 1 and x.shape[-1] == w.k, f"x has {w.k} columns")
+        _need(x.device == w.codes.device, f"x must be on {w.codes.device}")
+        if b is not None:
+            _typed(b, torch.bfloat16, "b")
+            _need(b.shape == (w.n,) and b.is_contiguous() and b.device == x.device, f"b is [{w.n}], contiguous")
+        if not w.cuda:
+            return ref.linear4(x, w, b)
+        if x.numel() == 0:
+            return x.new_empty(*x.shape[:-1], w.n)
+        rows = x.reshape(-1, w.k).clone(memory_format=torch.contiguous_format)     # whole rows at 16 bytes
+        return linear4(rows, w, b).view(*x.shape[:-1], w.n)
+    M, ld, y, dev = fast
+    with _there(dev):
+        check(kernels().loqa_linear4(x, ld, w.codes, w.scales, w.zeros, b, y, w.n, M, w.n, w.k, w.group, _stream(dev)), "linear4")
     return y
