@@ -3,14 +3,15 @@
 //
 // Bound by the bytes of the codes, which each wave streams as whole kilobytes: 16 features by 128 columns, laid out
 // once as the MFMA wants them (shuffle4 below), a lane's 16 bytes the codes of its feature for four MFMAs. Codes become
-// bf16 without arithmetic: 0x4300 | c is 128 + c exactly, so a pair of them costs an AND-OR and a shift. The group's
-// sum then is
+// bf16 without arithmetic: 0x4300 | c is 128 + c exactly, so a pair of them costs an AND-OR and a shift. What that adds to a
+// group's sum is taken off by a second MFMA whose weights are all -(128 + z), exact as well:
 //
-//   sum_k (128 + c) x  =  sum_k (c - z) x  +  (128 + z) sum_k x,
+//   sum_k (128 + c) x  +  sum_k -(128 + z) x  =  sum_k (c - z) x,
 //
-// of which the second part is taken off in f32, with sum_k x from one more MFMA of ones (shared by a wave's
-// features), before the scale; products of whole numbers up to 143 with bf16 are exact, and what f32 sums lose, 2^-24
+// and the group's scale enters in f32. Products of whole numbers up to 143 with bf16 are exact, and what f32 sums lose, 2^-24
 // of terms up to 143 |x| where the result's own are up to 15 |x|, is far below the result's rounding to bf16.
+// (With sums of x from an MFMA of ones and the subtraction in f32, vector instructions bounded small groups: 28672 x 4096 for
+// eight rows in groups of 64 with zeros 20 us, 17 now.)
 // The waves of a workgroup share its features and divide K; they meet in LDS.
 #include "common.h"
 
@@ -38,28 +39,33 @@ __global__ __launch_bounds__(256) void shuffle4_kernel(const unsigned char* src,
   dst[id] = w;
 }
 
-// [N, groups] -> [tile][group][16], zeros past N
-template <typename T> __global__ __launch_bounds__(256) void shuffle4_groups_kernel(const T* src, T* dst, int N, int groups, long long total) {
+// Scales [N, groups] -> [tile][K block][fq][group of the block][4]: a lane's four features (4 fq ..) of all groups side by side;
+// zeros -> [tile][K block][feature][group of the block] as -(128 + z)'s lower byte, z. Zeros past N and K.
+template <typename T, bool QUADS> __global__ __launch_bounds__(256) void shuffle4_groups_kernel(const T* src, T* dst, int N, int groups, int per,
+                                                                                               int blocks, long long total) {
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
   if (id >= total) return;
-  const long long tg = id >> 4;
-  const int n = (int)(tg / groups) * L4_TILE + (int)(id & 15), g = (int)(tg % groups);
-  dst[id] = n < N ? src[(size_t)n * groups + g] : (T)0;
+  const int in = (int)(id % (16 * per));
+  const long long tb = id / (16 * per);
+  const int f = QUADS ? in / (4 * per) * 4 + in % 4 : in / per, g = (int)(tb % blocks) * per + (QUADS ? in / 4 % per : in % per);
+  const long long n = tb / blocks * L4_TILE + f;
+  dst[id] = n < N && g < groups ? src[n * groups + g] : (T)0;
 }
 
 extern "C" int loqa_shuffle4(const void* codes, const void* scales, const void* zeros, void* dst, void* dst_scales, void* dst_zeros, int N, int K,
                              int group, hipStream_t st) {
   if (N <= 0 || K <= 0 || K % 32 || (group != 32 && group != 64 && group != 128) || K % group) return (int)hipErrorInvalidValue;
   const long long tiles = (N + L4_TILE - 1) / L4_TILE, blocks = (K + L4_K - 1) / L4_K, groups = K / group;
-  const long long total = tiles * blocks * 256, per = tiles * groups * 16;
+  const int in_block = L4_K / group;
+  const long long total = tiles * blocks * 256, per = tiles * blocks * in_block * 16;
   if ((total + 255) / 256 > 1LL << 30) return (int)hipErrorInvalidValue;
   hipLaunchKernelGGL(shuffle4_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, (const unsigned char*)codes, (unsigned*)dst, N, K,
                      (int)blocks, total);
-  hipLaunchKernelGGL((shuffle4_groups_kernel<bf16_t>), dim3((unsigned)((per + 255) / 256)), dim3(256), 0, st, (const bf16_t*)scales,
-                     (bf16_t*)dst_scales, N, (int)groups, per);
+  hipLaunchKernelGGL((shuffle4_groups_kernel<bf16_t, true>), dim3((unsigned)((per + 255) / 256)), dim3(256), 0, st, (const bf16_t*)scales,
+                     (bf16_t*)dst_scales, N, (int)groups, in_block, (int)blocks, per);
   if (zeros)
-    hipLaunchKernelGGL((shuffle4_groups_kernel<unsigned char>), dim3((unsigned)((per + 255) / 256)), dim3(256), 0, st, (const unsigned char*)zeros,
-                       (unsigned char*)dst_zeros, N, (int)groups, per);
+    hipLaunchKernelGGL((shuffle4_groups_kernel<unsigned char, false>), dim3((unsigned)((per + 255) / 256)), dim3(256), 0, st,
+                       (const unsigned char*)zeros, (unsigned char*)dst_zeros, N, (int)groups, in_block, (int)blocks, per);
   return (int)hipGetLastError();
 }
 
@@ -75,71 +81,126 @@ struct Linear4Args {
   int M, N, K;
 };
 
-// MT: tiles of 16 rows of x; GS: MFMAs (of 32 columns) a group
-template <int MT, int GS, bool Z, int NW>
+// MT: tiles of 16 rows of x; FT: tiles of features of a wave, which share its x; GS: MFMAs (of 32 columns) a group. A block's
+// codes, scales and zeros are asked for while the block before is worked on, and the x of one tile of rows.
+template <int MT, int FT, int GS, bool Z> struct L4Block {
+  static constexpr int NG = 4 / GS;
+  l4_u4 c[FT];
+  unsigned s[FT][2 * NG], z[FT];
+  bf16x8 x[MT == 1 ? 4 : 1];
+};
+
+// a wave-uniform address and a lane's offset, as the loads take them (64-bit sums a lane were a tenth of the loop)
+template <typename T> __device__ __forceinline__ T l4_at(const void* base, unsigned off) {
+  return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + off);
+}
+
+template <int MT, int FT, int GS, bool Z, int NW>
 __global__ __launch_bounds__(NW * 64) void linear4_kernel(Linear4Args A) {
-  __shared__ float4v sums[NW][MT][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, fq = lane >> 4;
-  const int tile = blockIdx.x, m0 = blockIdx.y * (16 * MT), blocks = (A.K + L4_K - 1) / L4_K, groups = A.K / (32 * GS);
-  const l4_u4* w = A.w + ((size_t)tile * blocks) * 64 + lane;
-  const bf16_t* sp = A.scales + (size_t)tile * groups * 16 + 4 * fq;
-  const unsigned char* zp = A.zeros + (size_t)tile * groups * 16 + 4 * fq;
+  using Block = L4Block<MT, FT, GS, Z>;
+  constexpr int NG = Block::NG;
+  __shared__ float4v sums[NW][FT][MT][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, fq = lane >> 4;
+  const int tiles = (A.N + L4_TILE - 1) / L4_TILE, tile0 = blockIdx.x * FT, m0 = blockIdx.y * (16 * MT);
+  const int blocks = (A.K + L4_K - 1) / L4_K;
   const bf16_t* xp[MT];                           // rows behind the last one read the last
 #pragma unroll
   for (int t = 0; t < MT; ++t) xp[t] = A.x + (size_t)min(m0 + 16 * t + li, A.M - 1) * A.ldx + 8 * fq;
-  bf16x8 ones;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) ones[j] = (__bf16)1.0f;
+  unsigned magic = 0x43004300u;                   // in a vector register: an AND-OR takes one constant from elsewhere
+  asm volatile("" : "+v"(magic));
   const float4v zero = {0.f, 0.f, 0.f, 0.f};
-  float4v acc[MT];
+  float4v acc[FT][MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = zero;
-  for (int kb = wave; kb < blocks; kb += NW) {
-    const l4_u4 c = w[(size_t)kb * 64];
-    float4v part[MT], xs[MT];
+  for (int f = 0; f < FT; ++f)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[f][t] = zero;
+  auto xread = [&](int t, int kb, int s) __attribute__((always_inline)) { return *reinterpret_cast<const bf16x8*>(xp[t] + min(kb * L4_K + 32 * s, A.K - 32)); };
+  auto load = [&](Block& b, int kb) __attribute__((always_inline)) {
+    kb = min(kb, blocks - 1);
+#pragma unroll
+    for (int f = 0; f < FT; ++f) {                // tiles behind the last one read the last
+      const size_t at = (size_t)min(tile0 + f, tiles - 1) * blocks + kb;
+      b.c[f] = l4_at<l4_u4>(A.w + at * 64, lane * 16);
+      if constexpr (NG == 1) {
+        const uint2 v = l4_at<uint2>(A.scales + at * 16, fq * 8);
+        b.s[f][0] = v.x; b.s[f][1] = v.y;
+      } else {
+#pragma unroll
+        for (int g = 0; g < NG; g += 2) {
+          const uint4 v = l4_at<uint4>(A.scales + at * (16 * NG), fq * (8 * NG) + g * 8);
+          b.s[f][2 * g] = v.x; b.s[f][2 * g + 1] = v.y; b.s[f][2 * g + 2] = v.z; b.s[f][2 * g + 3] = v.w;
+        }
+      }
+      if constexpr (Z && NG == 1) b.z[f] = l4_at<unsigned char>(A.zeros + at * 16, li);
+      if constexpr (Z && NG == 2) b.z[f] = l4_at<unsigned short>(A.zeros + at * 32, li * 2);
+      if constexpr (Z && NG == 4) b.z[f] = l4_at<unsigned>(A.zeros + at * 64, li * 4);
+    }
+    if constexpr (MT == 1) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) b.x[s] = xread(0, kb, s);
+    }
+  };
+  auto work = [&](const Block& b, int kb) __attribute__((always_inline)) {
+    bf16x8 x[MT][4];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        if constexpr (MT == 1) x[t][s] = b.x[s];
+        else x[t][s] = xread(t, kb, s);
+      }
+    float4v part[FT][MT];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const int k = kb * L4_K + 32 * s;
-      if (k >= A.K) break;                        // uniform
-      if (s % GS == 0) {
+      if (kb * L4_K + 32 * s >= A.K) break;       // uniform
+      const int g = s / GS;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) part[t] = xs[t] = zero;
-      }
-      l4_u4 b;
-#pragma unroll
-      for (int p = 0; p < 4; ++p) b[p] = ((c[s] >> (4 * p)) & 0x000f000fu) | 0x43004300u;
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const bf16x8 xf = *reinterpret_cast<const bf16x8*>(xp[t] + k);
-        part[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), xf, part[t], 0, 0, 0);
-        xs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, xf, xs[t], 0, 0, 0);
-      }
-      if (s % GS == GS - 1) {
-        const int g = k / (32 * GS);
-        const uint2 sc = *reinterpret_cast<const uint2*>(sp + (size_t)g * 16);
-        const float4v scale = {__uint_as_float(sc.x << 16), __uint_as_float(sc.x & 0xffff0000u), __uint_as_float(sc.y << 16), __uint_as_float(sc.y & 0xffff0000u)};
-        float4v off = {136.f, 136.f, 136.f, 136.f};
+      for (int f = 0; f < FT; ++f) {
+        l4_u4 w, minus = {0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};      // -136
         if constexpr (Z) {
-          const unsigned z = *reinterpret_cast<const unsigned*>(zp + (size_t)g * 16);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) off[j] = 128.f + (float)((z >> (8 * j)) & 255u);
+          const unsigned z = (b.z[f] >> (8 * g)) & 255u, m = z | z << 16 | 0xc300c300u;
+          minus = l4_u4{m, m, m, m};
         }
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int p = 0; p < 4; ++p) w[p] = ((b.c[f][s] >> (4 * p)) & 0x000f000fu) | magic;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[t][j] = fmaf(scale[j], fmaf(-off[j], xs[t][j], part[t][j]), acc[t][j]);
+        for (int t = 0; t < MT; ++t) {
+          part[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, minus), x[t][s], s % GS == 0 ? zero : part[f][t], 0, 0, 0);
+          part[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), x[t][s], part[f][t], 0, 0, 0);
+        }
+        if (s % GS == GS - 1) {
+          const unsigned s0 = b.s[f][2 * g], s1 = b.s[f][2 * g + 1];
+          const float4v scale = {__uint_as_float(s0 << 16), __uint_as_float(s0 & 0xffff0000u), __uint_as_float(s1 << 16), __uint_as_float(s1 & 0xffff0000u)};
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[f][t][j] = fmaf(scale[j], part[f][t][j], acc[f][t][j]);
+        }
       }
+    }
+  };
+  if (wave < blocks) {
+    Block a, b;
+    load(a, wave);
+    for (int kb = wave; kb < blocks; kb += 2 * NW) {
+      load(b, kb + NW);
+      work(a, kb);
+      if (kb + NW >= blocks) break;
+      load(a, kb + 2 * NW);
+      work(b, kb + NW);
     }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) sums[wave][t][lane] = acc[t];
+  for (int f = 0; f < FT; ++f)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) sums[wave][f][t][lane] = acc[f][t];
   __syncthreads();
-  for (int id = tid; id < MT * 64; id += NW * 64) {
-    const int t = id >> 6, l = id & 63, row = m0 + 16 * t + (l & 15), n = tile * L4_TILE + 4 * (l >> 4);
+  for (int id = tid; id < FT * MT * 64; id += NW * 64) {
+    const int f = id / (MT * 64), t = (id >> 6) % MT, l = id & 63, row = m0 + 16 * t + (l & 15), n = (tile0 + f) * L4_TILE + 4 * (l >> 4);
     float4v o = zero;
 #pragma unroll
     for (int v = 0; v < NW; ++v) {
-      const float4v a = sums[v][t][l];
+      const float4v a = sums[v][f][t][l];
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] += a[j];
     }
@@ -158,17 +219,29 @@ __global__ __launch_bounds__(NW * 64) void linear4_kernel(Linear4Args A) {
   }
 }
 
-template <int MT, int GS> static void l4_go(const Linear4Args& a, hipStream_t st) {
-  constexpr int NW = 8;
-  const dim3 grid((a.N + L4_TILE - 1) / L4_TILE, (a.M + 16 * MT - 1) / (16 * MT));
-  if (a.zeros) hipLaunchKernelGGL((linear4_kernel<MT, GS, true, NW>), grid, dim3(NW * 64), 0, st, a);
-  else hipLaunchKernelGGL((linear4_kernel<MT, GS, false, NW>), grid, dim3(NW * 64), 0, st, a);
+template <int MT, int FT, int GS, int NW> static void l4_go(const Linear4Args& a, hipStream_t st) {
+  const int tiles = (a.N + L4_TILE - 1) / L4_TILE;
+  const dim3 grid((tiles + FT - 1) / FT, (a.M + 16 * MT - 1) / (16 * MT));
+  if (a.zeros) hipLaunchKernelGGL((linear4_kernel<MT, FT, GS, true, NW>), grid, dim3(NW * 64), 0, st, a);
+  else hipLaunchKernelGGL((linear4_kernel<MT, FT, GS, false, NW>), grid, dim3(NW * 64), 0, st, a);
+}
+
+// Features of a wave and waves of a workgroup. A wave of four tiles reads its x a quarter as often and has four kilobytes under
+// way; of one, there are four times as many workgroups. us by (tiles a wave, waves), cold weights, launches in a replayed graph:
+// 1 row x 28672 x 4096 (groups of 128) 20.8 (1, 8), 17.1 (2, 8), 16.6 (4, 8), 15.0 (4, 4); 8 rows (64, zeros) 28.2, 20.8, 19.9, 17.0;
+// 4 x 12288 x 4096 11.6, 10.8, 9.8, 9.5; 4 x 8192 x 4096 7.7, 6.3, 8.4, 9.0; 1 x 4096 x 4096 4.4, 5.3, 7.4, 7.7; 32 rows x 14336 x
+// 4096 36.1, 21.7, 15.8, 20.5; 64 rows 64.2, 37.3, 23.4, 27.6, x 4096 x 4096 17.7, 18.5, 20.8, 25.8.
+template <int MT, int GS> static void l4_features(const Linear4Args& a, hipStream_t st) {
+  const int tiles = (a.N + L4_TILE - 1) / L4_TILE;
+  if (tiles >= 640) return l4_go<MT, 4, GS, MT == 1 ? 4 : 8>(a, st);
+  if (tiles >= 384) return l4_go<MT, 2, GS, 8>(a, st);
+  l4_go<MT, 1, GS, 8>(a, st);
 }
 
 template <int MT> static void l4_group(const Linear4Args& a, int group, hipStream_t st) {
-  if (group == 32) l4_go<MT, 1>(a, st);
-  else if (group == 64) l4_go<MT, 2>(a, st);
-  else l4_go<MT, 4>(a, st);
+  if (group == 32) l4_features<MT, 1>(a, st);
+  else if (group == 64) l4_features<MT, 2>(a, st);
+  else l4_features<MT, 4>(a, st);
 }
 
 extern "C" int loqa_linear4(const void* x, long ldx, const void* w, const void* scales, const void* zeros, const void* bias, void* y, long ldy, int M,

@@ -347,8 +347,9 @@ class Weight4:
             return
         tiles, blocks = -(-self.n // 16), -(-self.k // 128)
         self.codes = torch.empty(tiles * blocks * 256, dtype=torch.int32, device=codes.device)
-        self.scales = torch.empty(tiles * groups * 16, dtype=torch.bfloat16, device=codes.device)
-        self.zeros = None if zeros is None else torch.empty(tiles * groups * 16, dtype=torch.uint8, device=codes.device)
+        padded = tiles * blocks * (128 // self.group) * 16
+        self.scales = torch.empty(padded, dtype=torch.bfloat16, device=codes.device)
+        self.zeros = None if zeros is None else torch.empty(padded, dtype=torch.uint8, device=codes.device)
         with _there(codes.get_device()):
             check(kernels().loqa_shuffle4(ptr(codes), ptr(scales), ptr(zeros), ptr(self.codes), ptr(self.scales), ptr(self.zeros), self.n, self.k,
                                           self.group, stream_ptr(codes)), "shuffle4")
