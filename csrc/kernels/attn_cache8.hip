@@ -192,16 +192,28 @@ __device__ __forceinline__ a8_u4 a8_raw(const unsigned char* base, unsigned byte
 }
 template <int N> __device__ __forceinline__ void a8_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-template <int D> struct A8Token {
+// R: stages of a wave's ring; one where no wave has a second tile, so that twice as many workgroups fit a compute unit
+template <int D, int R> struct A8Token {
   static constexpr int TB = A8_TILE * D, STAGE = 2 * TB + 256;         // K, V, a dword a lane of scales
-  static constexpr int RING = 2 * STAGE;
+  static constexpr int RING = R * STAGE;
   static constexpr int MERGE = A8_WAVES * A8_ROWS * (D + 4 + 2) * 4 + 16;
   static constexpr int SMEM = A8_WAVES * RING > MERGE ? A8_WAVES * RING : MERGE;
+  static constexpr int FIT = 163840 / SMEM < 4 ? 163840 / SMEM : 4;    // workgroups of a compute unit
 };
 
-template <int D, int KIND>
-__global__ __launch_bounds__(A8_WAVES * 64) void attn8_token_kernel(Attn8Args A) {
-  using L = A8Token<D>;
+__device__ __forceinline__ float a8_max16(float x) {    // over lane and lane ^ 16
+  const a8_u2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ float a8_sum16(float x) {
+  const a8_u2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <int D, int KIND, int R>
+__global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_token_kernel(Attn8Args A) {
+  using L = A8Token<D, R>;
   constexpr int LPR = D / 16, RPL = 64 / LPR, NL = A8_TILE / RPL;      // lanes a row, rows a load, loads of K (and of V)
   constexpr int NS = D / 64, ND = D / 16, LD = D + 4;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[L::SMEM];
@@ -216,133 +228,149 @@ __global__ __launch_bounds__(A8_WAVES * 64) void attn8_token_kernel(Attn8Args A)
   const int kt0 = (part * each + wave) * A8_TILE;
   constexpr int STEP = A8_WAVES * A8_TILE;
   const int* bt = A.bt + (size_t)b * A.max_blocks;
-  auto page_at = [&](int kt, int i) { return a8_scalar(bt + min((kt + 16 * i) >> A.sh, A.max_blocks - 1)); };
+  auto page_at = [&](int kt) { return a8_scalar(bt + min(kt >> A.sh, A.max_blocks - 1)); };
+  // page numbers of the tile asked for next and of the one behind it
+  int pa0 = page_at(kt0), pa1 = page_at(kt0 + 16), pb0 = R > 1 ? page_at(kt0 + STEP) : 0, pb1 = R > 1 ? page_at(kt0 + STEP + 16) : 0;
 
-  // the queries of row li: K slots (fq, e) of MFMAs 2 s and 2 s + 1 are columns 64 s + 16 fq + e and + 8 + e
+  // the queries of row li, asked for ahead of the first tile: K slots (fq, e) of MFMAs 2 s and 2 s + 1 are columns 64 s + 16 fq + e
+  // and + 8 + e
   const int tok = li / Gq;
-  c8_h8 qf[2 * NS];
-  float factor;
+  const bool row = li < rows;
+  uint4 x[2 * NS];
   {
-    const bool row = li < rows;
     const bf16_t* qp = A.q + (size_t)(f.q0 + (row ? tok : 0)) * A.ldq + (size_t)(kvh * Gq + (row ? li - tok * Gq : 0)) * D + 16 * fq;
-    uint4 x[2 * NS];
     a8_row(A, x, [&](int u) { return qp + u / 2 * 64 + u % 2 * 8; });
-    float top = a8_top(x);
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const int e = a8_lift(top);
-    factor = ldexpf(A.scale_log2, -e);
-    a8_queries(x, row, e, false, qf);
-#pragma unroll
-    for (int u = 0; u < 2 * NS; ++u) asm volatile("" : "+v"(qf[u]));   // here before the loads whose count the compiler does not know
-    asm volatile("" : "+v"(factor));
   }
-  const int qpos = A.causal ? f.past + tok : 0x7fffffff;
+  const int qpos = A.causal ? f.past + tok : 0x7fffffff, seen = min(qpos, kend - 1);
 
   // chunk (16 codes) c of row r lies at place c ^ swz(r)
   auto swz = [](int row) { return D == 64 ? (row >> 1) & 3 : row & 7; };
-  unsigned voff[NL];
+  unsigned voff[NL / 2];
 #pragma unroll
-  for (int j = 0; j < NL; ++j) {
+  for (int j = 0; j < NL / 2; ++j) {
     const int r = j * RPL + lane / LPR;
-    voff[j] = (r & 15) * D + (((lane % LPR) ^ swz(r)) * 16);
+    voff[j] = r * D + (((lane % LPR) ^ swz(r)) * 16);
   }
   const unsigned ring = (unsigned)(size_t)(A8_LDS unsigned char*)lds + wave * L::RING;
   // A tile's loads (as many, where it has none, that reach nothing: the wait counts stay the same), 16 rows at a time, which a
   // page holds whole. The scales: lanes 0, 1 of the keys' two pages, 2, 3 of the values'.
-  auto ask = [&](int kt, unsigned slot, const int (&page)[2]) {
+  auto ask = [&](int kt, unsigned slot, int p0, int p1) __attribute__((always_inline)) {
     const int n = min(max(kend - kt, 0), A8_TILE);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int at = kt + 16 * t;
-      const bool there = (unsigned)page[t] < (unsigned)A.n_blocks;
-      const size_t off = ((((size_t)(there ? page[t] : 0) * A.G + kvh) << A.sh) + (at & ((1 << A.sh) - 1))) * D;
+      const int at = kt + 16 * t, page = t ? p1 : p0;
+      const bool there = (unsigned)page < (unsigned)A.n_blocks;
+      const size_t off = ((((size_t)(there ? page : 0) * A.G + kvh) << A.sh) + (at & ((1 << A.sh) - 1))) * D;
       const unsigned bytes = there ? min(max(n - 16 * t, 0), 16) * D : 0;
       const a8_u4 rk = a8_raw(A.k + off, bytes), rv = a8_raw(A.v + off, bytes);
 #pragma unroll
-      for (int j = t * (NL / 2); j < (t + 1) * (NL / 2); ++j) {
-        a8_load16(rk, voff[j], slot + j * 1024);
-        a8_load16(rv, voff[j], slot + L::TB + j * 1024);
+      for (int j = 0; j < NL / 2; ++j) {
+        a8_load16(rk, voff[j], slot + (t * (NL / 2) + j) * 1024);
+        a8_load16(rv, voff[j], slot + L::TB + (t * (NL / 2) + j) * 1024);
       }
     }
-    const int p = lane & 1 ? page[1] : page[0];
+    const int p = lane & 1 ? p1 : p0;
     a8_load4((lane & 2 ? A.vs : A.ks) + ((unsigned)p < (unsigned)A.n_blocks ? (size_t)p * A.G + kvh : 0), slot + 2 * L::TB);
   };
   constexpr int LOADS = 2 * NL + 1;
   static_assert(NL >= 2 && NL % 2 == 0, "whole loads of 16 rows");
+  ask(kt0, ring, pa0, pa1);
+  if constexpr (R > 1) ask(kt0 + STEP, ring + L::STAGE, pb0, pb1);
 
+  // (waits for the rows, and with them for the tiles behind, which the compiler does not count)
+  c8_h8 qf[2 * NS];
+  float factor;
+  {
+    const int e = a8_lift(a8_max16(fl_max32(a8_top(x))));
+    factor = ldexpf(A.scale_log2, -e);
+    a8_queries(x, row, e, false, qf);
+  }
+  unsigned kat[NS], vat[ND];                     // places of the fragments in a stage
+#pragma unroll
+  for (int s = 0; s < NS; ++s) kat[s] = ring + li * D + (((4 * s + fq) ^ swz(li)) * 16);
+  // lane i of 16 names row i / 2 of its eight (keys 4 fq .. + 3 of both halves), bytes 8 (i % 2) ..; it gets column i
+#pragma unroll
+  for (int d = 0; d < ND; ++d) {
+    const int r = 16 * (li >> 3) + 4 * fq + ((li >> 1) & 3);
+    vat[d] = ring + L::TB + r * D + ((d ^ swz(r)) * 16) + (li & 1) * 8;
+  }
   float4v acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = float4v{0.f, 0.f, 0.f, 0.f};
   float m_run = A8_NONE, l_run = 0.f;
-  int pages[2][2] = {{page_at(kt0, 0), page_at(kt0, 1)}, {page_at(kt0 + STEP, 0), page_at(kt0 + STEP, 1)}};
-  ask(kt0, ring, pages[0]);
-  ask(kt0 + STEP, ring + L::STAGE, pages[1]);
-  unsigned slot = ring;
+  unsigned slot = 0;
   for (int kt = kt0; kt < kend; kt += STEP) {
-    int next[2] = {page_at(kt + 2 * STEP, 0), page_at(kt + 2 * STEP, 1)};       // wanted behind this tile's work
-    a8_wait<LOADS>();                            // this tile is here, the next one's loads may be under way
-    const float4v sc = *a8_lds<float4v>(slot + 2 * L::TB);
+    int next0 = 0, next1 = 0;                    // wanted behind this tile's work
+    if constexpr (R > 1) { next0 = page_at(kt + 2 * STEP); next1 = page_at(kt + 2 * STEP + 16); }
+    a8_wait<(R - 1) * LOADS>();                  // this tile is here, the next one's loads may be under way
+    const float4v sc = *a8_lds<float4v>(ring + slot + 2 * L::TB);
+    c8_u4 kw[2 * NS];
+#pragma unroll
+    for (int u = 0; u < 2 * NS; ++u) kw[u] = *a8_lds<c8_u4>(kat[u >> 1] + slot + 16 * (u & 1) * D);
+    a8_v2i vw[ND];                               // asked for here, wanted behind the exponentials
+#pragma unroll
+    for (int d = 0; d < ND; ++d) vw[d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(a8_lds<a8_v2i>(vat[d] + slot));
     float4v st[2] = {float4v{0.f, 0.f, 0.f, 0.f}, float4v{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const c8_u4 w = *a8_lds<c8_u4>(slot + (16 * t + li) * D + (((4 * s + fq) ^ swz(16 * t + li)) * 16));
-        st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c8_widen8<KIND>(w[0], w[1]), qf[2 * s], st[t], 0, 0, 0);
-        st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c8_widen8<KIND>(w[2], w[3]), qf[2 * s + 1], st[t], 0, 0, 0);
-      }
+    for (int u = 0; u < 2 * NS; ++u) {
+      st[u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c8_widen8<KIND>(kw[u][0], kw[u][1]), qf[u & ~1], st[u & 1], 0, 0, 0);
+      st[u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c8_widen8<KIND>(kw[u][2], kw[u][3]), qf[u | 1], st[u & 1], 0, 0, 0);
+    }
     float mx = -INFINITY, inv[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const bool there = (unsigned)pages[0][t] < (unsigned)A.n_blocks;
-      const float vs = a8_least(sc[2 + t]), c = there ? factor * sc[t] : 0.f, lv = there ? __builtin_amdgcn_logf(vs) : -INFINITY;
-      inv[t] = there ? 1.f / vs : 0.f;
+      const bool there = (unsigned)(t ? pa1 : pa0) < (unsigned)A.n_blocks;
+      const float vs = a8_least(sc[2 + t]), c = there ? factor * a8_least(sc[t]) : 0.f, lv = there ? __builtin_amdgcn_logf(vs) : -INFINITY;
+      inv[t] = there ? __builtin_amdgcn_rcpf(vs) : 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = kt + 16 * t + 4 * fq + j;
-        float sv = fmaf(st[t][j], c, lv);
-        if (key >= kend || key > qpos) sv = -INFINITY;
-        st[t][j] = sv;
-        mx = fmaxf(mx, sv);
-      }
+      for (int j = 0; j < 4; ++j) st[t][j] = fmaf(st[t][j], c, lv);
     }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float m_new = fmaxf(m_run, mx), alpha = exp2f(m_run - m_new);
-    m_run = m_new;
+    if (kt + A8_TILE > kend || (A.causal && kt + A8_TILE - 1 > f.past)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (kt + 16 * t + 4 * fq + j > seen) st[t][j] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, st[j >> 2][j & 3]);
+    mx = a8_max16(fl_max32(mx));
+    if (__any(mx > m_run + 8.f)) {               // as in the prompt form
+      const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[d][j] *= alpha;
+    }
     c8_h8 p;
-    float ls = 0.f;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float e = exp2f(st[t][j] - m_new);
+        const float e = __builtin_amdgcn_exp2f(st[t][j] - m_run);
         sum += e;
         p[4 * t + j] = (_Float16)e;
       }
-      ls = fmaf(sum, inv[t], ls);
+      l_run = fmaf(sum, inv[t], l_run);          // of this lane's keys
     }
-    l_run = l_run * alpha + ls;                  // of this lane's keys
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      // lane i of 16 names row i / 2 of its eight (keys 4 fq .. + 3 of both halves), bytes 8 (i % 2) ..; it gets column i
-      const int row = 16 * (li >> 3) + 4 * fq + ((li >> 1) & 3);
-      const a8_v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(a8_lds<a8_v2i>(slot + L::TB + row * D + ((d ^ swz(row)) * 16) + (li & 1) * 8));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[d][j] *= alpha;
-      acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c8_widen8<KIND>(w[0], w[1]), p, acc[d], 0, 0, 0);
+    for (int d = 0; d < ND; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c8_widen8<KIND>(vw[d][0], vw[d][1]), p, acc[d], 0, 0, 0);
+    if constexpr (R > 1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot has been read
+      ask(kt + 2 * STEP, ring + slot, next0, next1);
+      pa0 = pb0; pa1 = pb1; pb0 = next0; pb1 = next1;
+      slot = slot ? 0 : L::STAGE;
+    } else if (kt + STEP < kend) {               // only where a context is longer than the bound that the host gave
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      pa0 = page_at(kt + STEP); pa1 = page_at(kt + STEP + 16);
+      ask(kt + STEP, ring, pa0, pa1);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot has been read
-    ask(kt + 2 * STEP, slot, next);
-    pages[0][0] = pages[1][0]; pages[0][1] = pages[1][1];
-    pages[1][0] = next[0]; pages[1][1] = next[1];
-    slot = slot == ring ? ring + L::STAGE : ring;
   }
   a8_wait<0>();                                  // no load into LDS outlives the loop
-  l_run += __shfl_xor(l_run, 16, 64);
-  l_run += __shfl_xor(l_run, 32, 64);
+  l_run = a8_sum16(fl_both32(l_run));
   __syncthreads();
   float* so = reinterpret_cast<float*>(lds);             // [wave][row][LD]
   float* sm = so + A8_WAVES * A8_ROWS * LD;              // [wave][m, l][row]
@@ -694,7 +722,8 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   }
 }
 
-// parts: of a sequence's keys at most; each: tiles of 64 keys of a prompt's part (the longer blocks have more parts)
+// parts: of a sequence's keys at most; each: tiles of 64 keys of a prompt's part (the longer blocks have more parts); of a token step 1
+// where a wave is expected to have one tile (parts * 128 keys bound the contexts), else 2
 extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const void* v, const void* ks, const void* vs, const void* cu,
                                const void* ctx, const void* bt, void* out, long ldo, int T, int B, int H, int G, int D, int blk, int n_blocks,
                                int max_blocks, int max_q, float scale, int causal, int kind, int parts, int each, void* ws, long ws_floats, void* tickets,
@@ -715,7 +744,8 @@ extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const voi
                     max_q, parts, causal, (int)blocks, each, parts == 1 && units <= 512, scale * 1.4426950408889634f};
   if (token) {
     const dim3 grid(parts, G, B);
-#define GO(D_, K_) hipLaunchKernelGGL((attn8_token_kernel<D_, K_>), grid, dim3(A8_WAVES * 64), 0, st, a)
+#define GO(D_, K_) do { if (each == 1) hipLaunchKernelGGL((attn8_token_kernel<D_, K_, 1>), grid, dim3(A8_WAVES * 64), 0, st, a); \
+                        else hipLaunchKernelGGL((attn8_token_kernel<D_, K_, 2>), grid, dim3(A8_WAVES * 64), 0, st, a); } while (0)
     if (D == 64) { if (kind == C8_INT8) GO(64, C8_INT8); else GO(64, C8_E4M3); }
     else { if (kind == C8_INT8) GO(128, C8_INT8); else GO(128, C8_E4M3); }
 #undef GO

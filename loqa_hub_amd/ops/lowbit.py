@@ -32,7 +32,7 @@ from ._lib import check, kernels, ptr, stream_ptr
 CACHE_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 HEAD_DIMS = (64, 128)
 TOKEN_ROWS, PROMPT_ROWS = 16, 128     # rows of a workgroup of the two forms (csrc/kernels/attn_cache8.hip)
-PROMPT_SLOTS = {64: 768, 128: 512}    # workgroups of the second that the chip holds, by head_dim
+TOKEN_SLOTS, PROMPT_SLOTS = {64: 512, 128: 256}, {64: 768, 128: 512}    # their workgroups at once, by head_dim
 
 
 def _need(ok: bool, what: str) -> None:
@@ -186,11 +186,14 @@ def read8(cache: Cache8, cu_k: torch.Tensor, first: torch.Tensor, block_tables: 
 
 @functools.lru_cache(maxsize=4096)
 def attn8_plan(max_q: int, group: int, units: int, keys: int, D: int) -> tuple[int, int, int, int]:
-    """(parts of a sequence's keys at most, tiles of 64 keys of a prompt's part, floats of workspace, tickets) for ``units``
+    """(parts of a sequence's keys at most, tiles of 64 keys of a prompt's part or stages of a token's ring, floats of workspace, tickets) for ``units``
     (sequence, kv head) pairs of up to ``max_q`` rows, ``group`` heads and ``keys`` keys."""
     if max_q * group <= TOKEN_ROWS:
-        parts = max(1, min(-(-512 // units), -(-keys // 128), 64))
-        return (parts, 1, units * parts * TOKEN_ROWS * (D + 2), units) if parts > 1 else (1, 1, 0, 0)
+        # a workgroup for each compute unit, two of 64 columns, and no part of less than a tile for each wave. us by parts: 1 context of
+        # 100000 x 8 heads of 128 86 (12), 53.5 (24), 47.6 (32), 53.9 (48), 56.3 (64); 32 of 4000 52.4 (1), 53.9 (2), 57.3 (4); 8 of
+        # 600 10.6 (1), 9.9 (5); 1 of 4000 41.1 (1), 12.1 (8), 11.3 (16, 32); 8 of 1500 x 20 of 64 15.4 (1), 13.3 (3), 14.2 (6)
+        parts = max(1, min(round(TOKEN_SLOTS[D] / units), -(-keys // 128)))
+        return (parts, 1 if keys <= 128 * parts else 2, *((units * parts * TOKEN_ROWS * (D + 2), units) if parts > 1 else (0, 0)))
     blocks, most = -(-max_q * group // PROMPT_ROWS), max(1, -(-keys // 64))
     parts = max(1, min(PROMPT_SLOTS[D] // (units * blocks), most // 4, 16))
     return (parts, -(-most // parts), units * blocks * parts * PROMPT_ROWS * (D + 4), units * blocks) if parts > 1 else (1, most, 0, 0)
