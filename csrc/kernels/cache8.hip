@@ -26,6 +26,7 @@ struct AppendArgs {
 };
 
 #define AP_HEADS 4                                // query heads of a thread
+#define AP_DEEP 4
 
 template <int D> struct ApPair {                  // entries c, c + 1, c + 2, c + 3 of both halves of a row
   float4v a, b;
@@ -94,21 +95,32 @@ __global__ __launch_bounds__(256) void rope_append8_kernel(AppendArgs A) {
   const bool turn = A.cs && !values;
   const int c = lane % LPR * 4, r0 = lane / LPR;
   const bf16_t* src = A.qkv + (size_t)(q0 + lo - start) * A.ld + (size_t)(A.H + (values ? A.G : 0) + g) * D;
-  auto row = [&](int r) {
-    ApPair<D> p = ap_load<D>(src + (size_t)r * A.ld, c);
-    if (turn) ap_rotate<D>(p, ap_turn<D>(A, lo + r, c));
-    return p;
-  };
-  // magnitudes as whole numbers: infinities and NaN are the largest
-  unsigned top = 0;
-  for (int r = r0; r < rows; r += RPW) {
-    const ApPair<D> p = row(r);
+  const unsigned had = off > 0 ? __float_as_uint(*scale) & 0x7fffffffu : 0u;
+  // AP_DEEP rows of a lane under way together; a page of no more than that is read once
+  constexpr int DEEP = AP_DEEP * RPW;
+  ApPair<D> p[AP_DEEP];
+  auto take = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, max(__float_as_uint(p.a[i]) & 0x7fffffffu, __float_as_uint(p.b[i]) & 0x7fffffffu));
+    for (int i = 0; i < AP_DEEP; ++i) p[i] = ap_load<D>(src + (size_t)min(at + i * RPW + r0, rows - 1) * A.ld, c);
+    if (turn) {
+      ApTurn t[AP_DEEP];
+#pragma unroll
+      for (int i = 0; i < AP_DEEP; ++i) t[i] = ap_turn<D>(A, lo + min(at + i * RPW + r0, rows - 1), c);
+#pragma unroll
+      for (int i = 0; i < AP_DEEP; ++i) ap_rotate<D>(p[i], t[i]);
+    }
+  };
+  // magnitudes as whole numbers: infinities and NaN are the largest (rows behind the last one are the last once more)
+  unsigned top = 0;
+  for (int at = 0; at < rows; at += DEEP) {
+    take(at);
+#pragma unroll
+    for (int u = 0; u < AP_DEEP; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = max(top, max(__float_as_uint(p[u].a[i]) & 0x7fffffffu, __float_as_uint(p[u].b[i]) & 0x7fffffffu));
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
-  const unsigned had = off > 0 ? __float_as_uint(*scale) & 0x7fffffffu : 0u;
   const unsigned now = max(max(c8_scale<KIND>(top), had), __float_as_uint(C8_LEAST));
   const float s = __uint_as_float(now), s_had = __uint_as_float(had);
   if (off > 0 && now != had)
@@ -120,10 +132,15 @@ __global__ __launch_bounds__(256) void rope_append8_kernel(AppendArgs A) {
       for (int i = 0; i < 4; ++i) { f[0][i] *= s_had; f[1][i] *= s_had; }
       *p = make_uint2(c8_codes<KIND>(f[0], s), c8_codes<KIND>(f[1], s));
     }
-  for (int r = r0; r < rows; r += RPW) {
-    const ApPair<D> p = row(r);
-    *reinterpret_cast<unsigned*>(codes + (off + r) * D + c) = c8_codes<KIND>(p.a, s);
-    *reinterpret_cast<unsigned*>(codes + (off + r) * D + D / 2 + c) = c8_codes<KIND>(p.b, s);
+  for (int at = 0; at < rows; at += DEEP) {
+    if (rows > DEEP) take(at);
+#pragma unroll
+    for (int i = 0; i < AP_DEEP; ++i) {
+      const int r = at + i * RPW + r0;
+      if (r >= rows) continue;
+      *reinterpret_cast<unsigned*>(codes + (off + r) * D + c) = c8_codes<KIND>(p[i].a, s);
+      *reinterpret_cast<unsigned*>(codes + (off + r) * D + D / 2 + c) = c8_codes<KIND>(p[i].b, s);
+    }
   }
   if (lane == 0 && (off == 0 || now != had)) *scale = s;
 }
@@ -217,7 +234,8 @@ extern "C" int loqa_read8(const void* k, const void* v, const void* ks, const vo
 // cu, first and given the sums of n, want and back ahead of i. Every workgroup sums up all sequences in LDS (a few
 // KB, from L2) and takes its part of the tokens, of the entries handed out and of those given back, each found by
 // bisection of the sums; a token's page follows from the ring itself, so nothing waits for the table. What a caller may
-// update in place (lengths, the ring's head and count) is written by the last workgroup to have read it.
+// update in place (lengths, the ring's head and count) is written by the last workgroup to have read it (without a ticket there
+// is one workgroup).
 // All or nothing: with a status nothing changes.
 struct PageArgs {
   const int *n, *ctx;
@@ -292,7 +310,8 @@ __global__ __launch_bounds__(PS_THREADS) void page_step_kernel(PageArgs A) {
   __syncthreads();
   bad = bad_s;
   // every workgroup is through with lengths and ring: the last one may write them
-  if (tid == 0) {
+  if (tid == 0 && gridDim.x == 1) last_s = 1;
+  else if (tid == 0) {
     const int t = __hip_atomic_fetch_add(A.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     last_s = t == (int)gridDim.x - 1;
     if (last_s) __hip_atomic_store(A.ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -354,7 +373,7 @@ extern "C" int loqa_page_step(const void* n, const void* ctx, void* table, void*
   if (B <= 0 || B > PS_SEQS || width <= 0 || blk <= 0 || (blk & (blk - 1)) || pool <= 0 || most < 0 || most > 1 << 30) return (int)hipErrorInvalidValue;
   const PageArgs a{(const int*)n, (const int*)ctx, (int*)table, (int*)free_, (const int*)ring, (int*)cu, (int*)pos, (int*)slots, (long long*)last,
                    (int*)ctx_out, (int*)ring_out, (int*)status, (int*)ticket, B, width, __builtin_ctz(blk), pool, most};
-  const int wgs = max(1, min(128, (most + 2 * PS_THREADS - 1) / (2 * PS_THREADS)));
+  const int wgs = ticket ? max(1, min(64, (most + PS_THREADS - 1) / PS_THREADS)) : 1;
   hipLaunchKernelGGL(page_step_kernel, dim3(wgs), dim3(PS_THREADS), 0, st, a);
   return (int)hipGetLastError();
 }

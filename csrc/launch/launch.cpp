@@ -10,8 +10,10 @@
 // types here with those it knows.
 #include <Python.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/narrow.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <exception>
 #include <string>
 #include <utility>
@@ -260,22 +262,92 @@ PyObject* cache8_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// (new_lens, ctx_lens, block_tables, free_pages, ring, ctx_out or None, ring_out or None; max_tokens) -> (B, columns, pool, cu_q,
-// positions, slots, last_rows, ctx_out, ring_out, status, device)
-PyObject* page_tensors(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  return checked<7, 1>(args, n, [](const at::Tensor* const* t, const long* v) -> PyObject* {
-    if (!t[2] || !t[2]->is_cuda()) Py_RETURN_NONE;
+// Whole calls: checks, allocations and the launch, where the tensors are on the current device; None as above.
+PyObject* launched(int rc, const char* what) {
+  if (rc != 0) PyErr_Format(PyExc_RuntimeError, "%s failed with hipError %d", what, rc);
+  return nullptr;
+}
+
+// (qkv, q_out or None, cu_q, ctx_lens, block_tables, cos_sin or None, k, v, k_scale, v_scale; heads, kv heads, columns, rows of a page,
+// pages, max_q, kind, current device, its stream) -> q
+PyObject* rope_append8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return checked<10, 9>(args, n, [](const at::Tensor* const* t, const long* v) -> PyObject* {
+    if (!t[0] || !t[6] || !t[6]->is_cuda() || t[6]->get_device() != v[7]) Py_RETURN_NONE;
+    const at::Tensor &x = *t[0], &bt = *t[4];
+    const at::Device dev = t[6]->device();
+    const long H = v[0], G = v[1], D = v[2];
+    if (!rows_on(x, (H + 2 * G) * D, dev) || (t[1] && (!rows_on(*t[1], H * D, dev) || t[1]->size(0) != x.size(0)))) Py_RETURN_NONE;
+    if (!i32_on(t[2], dev) || !i32_on(t[3], dev) || !i32_on(t[4], dev)) Py_RETURN_NONE;
+    const long T = x.size(0), B = t[3]->numel();
+    if (T == 0 || B == 0 || v[5] <= 0 || t[2]->numel() != B + 1 || bt.dim() != 2 || bt.size(0) != B || bt.size(1) == 0) Py_RETURN_NONE;
+    if (t[5] && (t[5]->scalar_type() != at::kFloat || t[5]->dim() != 3 || t[5]->size(1) * 2 != D || t[5]->size(2) != 2 || t[5]->size(0) == 0 ||
+                 !t[5]->is_contiguous() || t[5]->device() != dev || ((size_t)t[5]->data_ptr() & 15)))
+      Py_RETURN_NONE;
+    const at::Tensor q = t[1] ? *t[1] : made({T, H * D}, at::kBFloat16, dev);
+    if ((((size_t)x.data_ptr() | (size_t)q.data_ptr()) & 7) || ((x.stride(0) | q.stride(0)) & 3)) Py_RETURN_NONE;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = loqa_rope_append8(x.data_ptr(), x.stride(0), t[5] ? t[5]->data_ptr() : nullptr, t[5] ? (int)t[5]->size(0) : 0, t[6]->data_ptr(), t[7]->data_ptr(),
+                           t[8]->data_ptr(), t[9]->data_ptr(), t[2]->data_ptr(), t[3]->data_ptr(), bt.data_ptr(), q.data_ptr(), q.stride(0), (int)T,
+                           (int)B, (int)H, (int)G, (int)D, (int)v[3], (int)v[4], (int)bt.size(1), (int)std::min(v[5], T), (int)v[6], (stream_t)v[8]);
+    Py_END_ALLOW_THREADS
+    return rc ? launched(rc, "rope_append8") : THPVariable_Wrap(q);
+  });
+}
+
+// (cu_k, first, block_tables, k, v, k_scale, v_scale; kv heads, columns, rows of a page, pages, total, kind, current device, its stream)
+// -> (k, v)
+PyObject* read8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return checked<7, 8>(args, n, [](const at::Tensor* const* t, const long* v) -> PyObject* {
+    if (!t[3] || !t[3]->is_cuda() || t[3]->get_device() != v[6]) Py_RETURN_NONE;
+    const at::Device dev = t[3]->device();
+    if (!i32_on(t[0], dev) || !i32_on(t[1], dev) || !i32_on(t[2], dev)) Py_RETURN_NONE;
+    const at::Tensor& bt = *t[2];
+    const long B = t[1]->numel(), total = v[4];
+    if (B == 0 || total <= 0 || total >= 1L << 31 || t[0]->numel() != B + 1 || bt.dim() != 2 || bt.size(0) != B || bt.size(1) == 0) Py_RETURN_NONE;
+    const at::Tensor k = made({total, v[0], v[1]}, at::kBFloat16, dev), u = made({total, v[0], v[1]}, at::kBFloat16, dev);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = loqa_read8(t[3]->data_ptr(), t[4]->data_ptr(), t[5]->data_ptr(), t[6]->data_ptr(), t[0]->data_ptr(), t[1]->data_ptr(), bt.data_ptr(),
+                    k.data_ptr(), u.data_ptr(), (int)total, (int)B, (int)v[0], (int)v[1], (int)v[2], (int)v[3], (int)bt.size(1), (int)v[5],
+                    (stream_t)v[7]);
+    Py_END_ALLOW_THREADS
+    return rc ? launched(rc, "read8") : Py_BuildValue("NN", THPVariable_Wrap(k), THPVariable_Wrap(u));
+  });
+}
+
+// (new_lens, ctx_lens, block_tables, free_pages, ring, ctx_out or None, ring_out or None, tickets or None; rows of a page, max_tokens, sequences
+// at most, current device, its stream) -> (cu_q, positions, slots, last_rows, ctx_out, ring_out, status)
+PyObject* page_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return checked<8, 5>(args, n, [](const at::Tensor* const* t, const long* v) -> PyObject* {
+    if (!t[2] || !t[2]->is_cuda() || t[2]->get_device() != v[3]) Py_RETURN_NONE;
     const at::Device dev = t[2]->device();
     for (int i = 0; i < 7; ++i)
       if (i < 5 ? !i32_on(t[i], dev) : t[i] && !i32_on(t[i], dev)) Py_RETURN_NONE;
     const at::Tensor& bt = *t[2];
-    const long B = t[0]->numel(), pool = t[3]->numel(), most = v[0];
-    if (B == 0 || t[1]->numel() != B || bt.dim() != 2 || bt.size(0) != B || bt.size(1) == 0 || t[4]->numel() != 2 || pool == 0 || most < 0)
+    const long B = t[0]->numel(), pool = t[3]->numel(), P = v[0], most = v[1];
+    if (B == 0 || B > v[2] || t[1]->numel() != B || bt.dim() != 2 || bt.size(0) != B || bt.size(1) == 0 || t[4]->numel() != 2 || pool == 0)
       Py_RETURN_NONE;
+    if (most < 0 || most > 1L << 30 || P <= 0 || (P & (P - 1)) || pool * P >= 1L << 31) Py_RETURN_NONE;
     if ((t[5] && t[5]->numel() != B) || (t[6] && t[6]->numel() != 2)) Py_RETURN_NONE;
-    auto ints = [&](long m) { return THPVariable_Wrap(made({m}, at::kInt, dev)); };
-    return Py_BuildValue("lllNNNNNNNl", B, (long)bt.size(1), pool, ints(B + 1), ints(most), ints(most), THPVariable_Wrap(made({B}, at::kLong, dev)),
-                         t[5] ? THPVariable_Wrap(*t[5]) : ints(B), t[6] ? THPVariable_Wrap(*t[6]) : ints(2), ints(1), (long)dev.index());
+    // one allocation for all that is int32
+    const at::Tensor all = made({B + 1 + 2 * most + B + 2 + 1}, at::kInt, dev), last = made({B}, at::kLong, dev);
+    long at = 0;
+    auto ints = [&](long m) {
+      const at::Tensor x = all.narrow(0, at, m);
+      at += m;
+      return x;
+    };
+    const at::Tensor cu = ints(B + 1), pos = ints(most), slots = ints(most), status = ints(1), ctx = t[5] ? *t[5] : ints(B), ring = t[6] ? *t[6] : ints(2);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = loqa_page_step(t[0]->data_ptr(), t[1]->data_ptr(), bt.data_ptr(), t[3]->data_ptr(), t[4]->data_ptr(), cu.data_ptr(), pos.data_ptr(),
+                        slots.data_ptr(), last.data_ptr(), ctx.data_ptr(), ring.data_ptr(), status.data_ptr(), t[7] ? t[7]->data_ptr() : nullptr,
+                        (int)B, (int)bt.size(1), (int)P, (int)pool, (int)most, (stream_t)v[4]);
+    Py_END_ALLOW_THREADS
+    if (rc) return launched(rc, "page_step");
+    return Py_BuildValue("NNNNNNN", THPVariable_Wrap(cu), THPVariable_Wrap(pos), THPVariable_Wrap(slots), THPVariable_Wrap(last),
+                         THPVariable_Wrap(ctx), THPVariable_Wrap(ring), THPVariable_Wrap(status));
   });
 }
 
@@ -322,7 +394,9 @@ PyMethodDef methods[] = {
     {"qk_shapes", (PyCFunction)(void (*)(void))qk_shapes, METH_FASTCALL, nullptr},
     {"window_shapes", (PyCFunction)(void (*)(void))window_shapes, METH_FASTCALL, nullptr},
     {"cache8_rows", (PyCFunction)(void (*)(void))cache8_rows, METH_FASTCALL, nullptr},
-    {"page_tensors", (PyCFunction)(void (*)(void))page_tensors, METH_FASTCALL, nullptr},
+    {"rope_append8", (PyCFunction)(void (*)(void))rope_append8, METH_FASTCALL, nullptr},
+    {"read8", (PyCFunction)(void (*)(void))read8, METH_FASTCALL, nullptr},
+    {"page_step", (PyCFunction)(void (*)(void))page_step, METH_FASTCALL, nullptr},
     {"linear4_rows", (PyCFunction)(void (*)(void))linear4_rows, METH_FASTCALL, nullptr},
     {"signatures", signatures, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};

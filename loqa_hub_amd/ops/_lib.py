@@ -351,8 +351,8 @@ def _main_kernels() -> ctypes.CDLL:
 _LAUNCH = frozenset(("loqa_qk_prep_append", "loqa_window_attention", "loqa_window_attention_parts", "loqa_delta_prep",
                      "loqa_delta_scan", "loqa_seq_state_save", "loqa_gated_rmsnorm", "loqa_moe_route", "loqa_latent_attention",
                      "loqa_latent_kv", "loqa_latent_prefill", "loqa_sigmoid_gate", "loqa_head_product", "i32c", "f32c", "qk_shapes", "window_shapes",
-                     "loqa_rope_append8", "loqa_read8", "loqa_attention8", "loqa_page_step", "loqa_linear4", "cache8_rows", "page_tensors",
-                     "linear4_rows"))
+                     "loqa_rope_append8", "loqa_read8", "loqa_attention8", "loqa_page_step", "loqa_linear4", "cache8_rows", "linear4_rows",
+                     "rope_append8", "read8", "page_step"))
 _launch = None
 
 

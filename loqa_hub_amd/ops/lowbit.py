@@ -56,6 +56,15 @@ def _there(index: int):
     return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
+def _elsewhere(cache, fn, *args, **kw):
+    """The call once more with the cache's device as the current one; its checks have passed."""
+    index = cache.k.get_device()
+    if index == torch._C._cuda_getDevice():
+        raise RuntimeError(f"{fn.__name__} does not take this call")
+    with torch.cuda.device(index):
+        return fn(*args, **kw)
+
+
 _HERE = contextlib.nullcontext()
 _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
@@ -135,53 +144,49 @@ def rope_append8(qkv: torch.Tensor, cos_sin: torch.Tensor | None, cache: Cache8,
     position (rows past its end are turned by its last entry). ``max_q`` bounds the rows of a sequence. Rotated keys
     go to their codes without a rounding in between. Rows at positions below zero or past the block table are not
     appended. An infinite or NaN entry makes its page's scale so, and with it what attention gives for the page."""
+    if cache.cuda:
+        dev = torch._C._cuda_getDevice()
+        q = kernels().rope_append8(qkv, q_out, cu_q, ctx_lens, block_tables, cos_sin, cache.k, cache.v, cache.k_scale, cache.v_scale, n_heads,
+                                   cache.n_kv, cache.head_dim, cache.block_size, cache.n_blocks, max_q, cache.kind, dev, _stream(dev))
+        if q is not None:
+            return q
     H, G, D = n_heads, cache.n_kv, cache.head_dim
     _need(H > 0 and max_q >= 0, "n_heads and max_q")
     if cos_sin is not None:
         _typed(cos_sin, torch.float32, "cos_sin")
         _need(cos_sin.dim() == 3 and cos_sin.shape[1:] == (D // 2, 2) and cos_sin.shape[0] > 0 and cos_sin.is_contiguous()
-              and cos_sin.device == cache.device and cos_sin.data_ptr() % 16 == 0, "cos_sin is [max_pos, head_dim / 2, 2], contiguous")
-    fast = _rows8(qkv, q_out, cu_q, ctx_lens, block_tables, cache, (H + 2 * G) * D, H * D)
-    if fast is None:
-        _rows(qkv, (H + 2 * G) * D, "qkv", cache)
-        T = qkv.shape[0]
-        B, _ = _sequences(cu_q, ctx_lens, block_tables, cache)
-        if q_out is None:
-            q_out = torch.empty(T, H * D, dtype=torch.bfloat16, device=qkv.device)
-        _rows(q_out, H * D, "q_out", cache)
-        _need(q_out.shape[0] == T, "q_out has the rows of qkv")
-        return q_out if T == 0 or B == 0 or max_q == 0 else \
-            ref.rope_append8(qkv, cos_sin, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, q_out=q_out)
-    T, B, max_blocks, ld, ldq, q_out, dev = fast
-    if max_q == 0:
+              and cos_sin.device == cache.device and cos_sin.data_ptr() % 16 == 0, "cos_sin is [max_pos, head_dim / 2, 2], contiguous, at 16 bytes")
+    _rows(qkv, (H + 2 * G) * D, "qkv", cache)
+    T = qkv.shape[0]
+    B, _ = _sequences(cu_q, ctx_lens, block_tables, cache)
+    if q_out is None:
+        q_out = torch.empty(T, H * D, dtype=torch.bfloat16, device=qkv.device)
+    _rows(q_out, H * D, "q_out", cache)
+    _need(q_out.shape[0] == T, "q_out has the rows of qkv")
+    if T == 0 or B == 0 or max_q == 0:
         return q_out
-    _need((qkv.data_ptr() | q_out.data_ptr()) % 8 == 0 and (ld | ldq) % 4 == 0, "rows of qkv and q_out must start at 8 bytes")
-    with _there(dev):
-        check(kernels().loqa_rope_append8(
-            qkv, ld, cos_sin, 0 if cos_sin is None else cos_sin.shape[0], cache.k, cache.v, cache.k_scale, cache.v_scale, cu_q, ctx_lens,
-            block_tables, q_out, ldq, T, B, H, G, D, cache.block_size, cache.n_blocks, max_blocks, min(max_q, T), cache.kind, _stream(dev)),
-            "rope_append8")
-    return q_out
+    if not cache.cuda:
+        return ref.rope_append8(qkv, cos_sin, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, q_out=q_out)
+    _need((qkv.data_ptr() | q_out.data_ptr()) % 8 == 0 and (qkv.stride(0) | q_out.stride(0)) % 4 == 0, "rows of qkv and q_out must start at 8 bytes")
+    return _elsewhere(cache, rope_append8, qkv, cos_sin, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, q_out=q_out)
 
 
 def read8(cache: Cache8, cu_k: torch.Tensor, first: torch.Tensor, block_tables: torch.Tensor, *, total: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Cached rows as what they stand for: row cu_k[b] + i of the results, k and v [total, Hkv, D] bf16, is position
     first[b] + i of sequence b (a prefix that moves to a bf16 cache, or is looked at). Zeros from pages that do not exist;
     rows of no sequence are zeros too."""
-    B, max_blocks = _sequences(cu_k, first, block_tables, cache)
+    if cache.cuda:
+        dev = torch._C._cuda_getDevice()
+        kv = kernels().read8(cu_k, first, block_tables, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.n_kv, cache.head_dim, cache.block_size,
+                             cache.n_blocks, total, cache.kind, dev, _stream(dev))
+        if kv is not None:
+            return kv
+    B, _ = _sequences(cu_k, first, block_tables, cache)
     _need(0 <= total < 1 << 31, "total")
-    shape = (total, cache.n_kv, cache.head_dim)
-    k = torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device)
-    v = torch.empty_like(k)
-    if not cache.cuda:
-        return ref.read8(cache, cu_k, first, block_tables, k.zero_(), v.zero_())
-    if total == 0 or B == 0:
-        return k.zero_(), v.zero_()
-    dev = k.get_device()
-    with _there(dev):
-        check(kernels().loqa_read8(cache.k, cache.v, cache.k_scale, cache.v_scale, cu_k, first, block_tables, k, v, total, B, cache.n_kv,
-                                   cache.head_dim, cache.block_size, cache.n_blocks, max_blocks, cache.kind, _stream(dev)), "read8")
-    return k, v
+    if cache.cuda and total > 0 and B > 0:
+        return _elsewhere(cache, read8, cache, cu_k, first, block_tables, total=total)
+    k, v = (torch.zeros(total, cache.n_kv, cache.head_dim, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
+    return (k, v) if cache.cuda else ref.read8(cache, cu_k, first, block_tables, k, v)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -241,7 +246,7 @@ def attention8(q: torch.Tensor, cache: Cache8, cu_q: torch.Tensor, ctx_lens: tor
 
 
 # ------------------------------------------------------------------ pages of a step
-PAGE_STEP_SEQS = 4096
+PAGE_STEP_SEQS, PAGE_STEP_FEW = 4096, 512
 
 
 class PageStep(NamedTuple):
@@ -269,37 +274,36 @@ def page_step(new_lens: torch.Tensor, ctx_lens: torch.Tensor, block_tables: torc
     sequences and given back behind the last free one. ``ctx_out`` / ``ring_out`` may be ``ctx_lens`` / ``ring`` themselves.
     All or nothing: where the status is not 0, nothing changes and no token has a slot. At most 4096 sequences. A page that
     several sequences share must not be given back here."""
-    _need(0 <= max_tokens <= 1 << 30, "max_tokens")
-    fast = kernels().page_tensors(new_lens, ctx_lens, block_tables, free_pages, ring, ctx_out, ring_out, max_tokens) if block_tables.is_cuda else None
-    if fast is None:
-        _typed(block_tables, torch.int32, "block_tables")
-        for t, name in ((new_lens, "new_lens"), (ctx_lens, "ctx_lens"), (block_tables, "block_tables"), (free_pages, "free_pages"), (ring, "ring"),
-                        (ctx_out, "ctx_out"), (ring_out, "ring_out")):
-            if t is not None:
-                _i32(t, name, block_tables)
-        B, pool = new_lens.numel(), free_pages.numel()
-        _need(B > 0, "no sequences")
-        _need(ctx_lens.numel() == B and block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.shape[1] > 0, "ctx_lens [B], block_tables [B, max_blocks]")
-        _need(ring.numel() == 2 and pool > 0, "ring [2], free_pages [N]")
-        for t, n, name in ((ctx_out, B, "ctx_out"), (ring_out, 2, "ring_out")):
-            _need(t is None or t.numel() == n, f"{name} has {n} entries")
-    else:
-        B, width, pool = fast[:3]
-    _need(B <= PAGE_STEP_SEQS, f"at most {PAGE_STEP_SEQS} sequences")
+    if block_tables.is_cuda:
+        dev = torch._C._cuda_getDevice()
+        st = _stream(dev)
+        # what several workgroups share; the few tokens of a decoding step take one
+        tickets = _sk_workspace(block_tables.device, st, 1, 1)[1] if max_tokens > PAGE_STEP_FEW and block_tables.get_device() == dev else None
+        step = kernels().page_step(new_lens, ctx_lens, block_tables, free_pages, ring, ctx_out, ring_out, tickets, block_size, max_tokens,
+                                   PAGE_STEP_SEQS, dev, st)
+        if step is not None:
+            return PageStep._make(step)
+    _typed(block_tables, torch.int32, "block_tables")
+    for t, name in ((new_lens, "new_lens"), (ctx_lens, "ctx_lens"), (block_tables, "block_tables"), (free_pages, "free_pages"), (ring, "ring"),
+                    (ctx_out, "ctx_out"), (ring_out, "ring_out")):
+        if t is not None:
+            _i32(t, name, block_tables)
+    B, pool = new_lens.numel(), free_pages.numel()
+    _need(0 < B <= PAGE_STEP_SEQS, f"1 to {PAGE_STEP_SEQS} sequences")
+    _need(ctx_lens.numel() == B and block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.shape[1] > 0, "ctx_lens [B], block_tables [B, max_blocks]")
+    _need(ring.numel() == 2 and pool > 0, "ring [2], free_pages [N]")
     _need(block_size > 0 and block_size & (block_size - 1) == 0 and pool * block_size < 1 << 31, "block_size is a power of two, slots have 32 bits")
-    if fast is None:
-        def ints(n, dtype=torch.int32):
-            return torch.empty(n, dtype=dtype, device=block_tables.device)
-        step = PageStep(ints(B + 1), ints(max_tokens), ints(max_tokens), ints(B, torch.int64), ints(B) if ctx_out is None else ctx_out,
-                        ints(2) if ring_out is None else ring_out, ints(1))
-        return ref.page_step(new_lens, ctx_lens, block_tables, free_pages, ring, block_size, step)
-    step, dev = PageStep._make(fast[3:10]), fast[10]
-    st = _stream(dev)
-    with _there(dev):
-        _, tickets = _sk_workspace(block_tables.device, st, 1, 1)
-        check(kernels().loqa_page_step(new_lens, ctx_lens, block_tables, free_pages, ring, step.cu_q, step.positions, step.slots, step.last_rows,
-                                       step.ctx_lens, step.ring, step.status, tickets, B, width, block_size, pool, max_tokens, st), "page_step")
-    return step
+    _need(0 <= max_tokens <= 1 << 30, "max_tokens")
+    for t, n, name in ((ctx_out, B, "ctx_out"), (ring_out, 2, "ring_out")):
+        _need(t is None or t.numel() == n, f"{name} has {n} entries")
+    if block_tables.is_cuda:
+        with torch.cuda.device(block_tables.device):
+            _need(block_tables.get_device() != dev, "page_step does not take this call")
+            return page_step(new_lens, ctx_lens, block_tables, free_pages, ring, block_size=block_size, max_tokens=max_tokens, ctx_out=ctx_out, ring_out=ring_out)
+    ints = functools.partial(torch.empty, dtype=torch.int32)
+    step = PageStep(ints(B + 1), ints(max_tokens), ints(max_tokens), torch.empty(B, dtype=torch.int64), ints(B) if ctx_out is None else ctx_out,
+                    ints(2) if ring_out is None else ring_out, ints(1))
+    return ref.page_step(new_lens, ctx_lens, block_tables, free_pages, ring, block_size, step)
 
 
 # ------------------------------------------------------------------ 4-bit weights
