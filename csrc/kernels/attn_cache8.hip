@@ -423,6 +423,7 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
 // 32 x 32 x 16 MFMAs as the bf16 form does (flash_pipe.h: layouts and swizzles).
 #define A8P_ROWS 128
 #define A8P_KEYS 64
+#define A8P_PARTS 16
 
 template <int D> struct A8Prompt {
   static constexpr int K = A8P_KEYS * D * 2, STAGE = 2 * K;
@@ -498,19 +499,16 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     }
   };
   // piece q of the tile in registers: 8 codes, of keys or of values, widened and put where the fragments are read from
-  // (lanes of a row's upper half put their second part first: eight lanes then write to eight different 16-byte banks)
   constexpr int PIECES = 4 * N;
-  const bool upper = cc * 2 >= CH;
   unsigned put_at[4];                                        // K's and V's two parts in the first stage; rows further on keep the swizzle
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int sw = q & 2 ? fl_vswz<D>(cr) : fl_kswz<D>(cr);
-    put_at[q] = base + (q & 2 ? L::K : 0) + cr * (D * 2) + ((2 * cc + ((q & 1) ^ (int)upper)) ^ sw) * 16;
+    put_at[q] = base + (q & 2 ? L::K : 0) + cr * (D * 2) + ((2 * cc + (q & 1)) ^ sw) * 16;
   }
   auto store = [&](int q) __attribute__((always_inline)) {
     const uint4 w = q & 2 ? vw[q >> 2] : kw[q >> 2];
-    const bool second = (q & 1) != (int)upper;
-    *fl_lds<c8_h8>(put_at[q & 3] + (q >> 2) * (256 / CH) * D * 2) = c8_widen8<KIND>(second ? w.z : w.x, second ? w.w : w.y);
+    *fl_lds<c8_h8>(put_at[q & 3] + (q >> 2) * (256 / CH) * D * 2) = q & 1 ? c8_widen8<KIND>(w.z, w.w) : c8_widen8<KIND>(w.x, w.y);
   };
   static_assert(256 / CH % 16 == 0, "a thread's rows share a swizzle");
   auto store_scales = [&](int stage) __attribute__((always_inline)) {
@@ -667,7 +665,7 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   const bool whole = (((size_t)A.out | (size_t)A.ldo * 2) & 7) == 0;
   const int row = wave * 32 + (lane & 31);
   // Parts of a block's keys: each leaves its accumulators as they lie (16 bytes a lane, a kilobyte a wave), and the last to arrive
-  // adds up all of them, in order, its own from its registers.
+  // adds up all of them, in order.
   if (nparts > 1) {
     constexpr int PER = 256 * (NDT * 16 + 2) * 4;
     const auto rs = __builtin_amdgcn_make_buffer_rsrc(A.ws + unit * A.parts * (PER / 4), 0, A.parts * PER, 0x00020000);
@@ -680,30 +678,36 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(a8_u2, make_float2(m, l)), rs, part * PER + ml, 0, 16);
     if (!a8_last(A.tickets + unit * TICKET, nparts, reinterpret_cast<int*>(lds))) return;
     float top = A8_NONE, all = 0.f;
-    for (int p = 0; p < nparts; ++p) top = fmaxf(top, __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, p * PER + ml, 0, 16)).x);
-    float16v total[NDT];
+    float tops[A8P_PARTS];                                   // all asked for together
 #pragma unroll
-    for (int d = 0; d < NDT; ++d) total[d] = zero;
-    for (int p = 0; p < nparts; ++p) {
-      const float2 w = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, p * PER + ml, 0, 16));
-      float4v v[4 * NDT];
-      if (p != part) {
+    for (int p = 0; p < A8P_PARTS; ++p) tops[p] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, min(p, nparts - 1) * PER + ml, 0, 16));
 #pragma unroll
-        for (int u = 0; u < 4 * NDT; ++u) v[u] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(rs, p * PER + tid * 16 + u * 4096, 0, 16));
-      } else {
+    for (int p = 0; p < A8P_PARTS; ++p) top = fmaxf(top, tops[p]);
 #pragma unroll
-        for (int u = 0; u < 4 * NDT; ++u) v[u] = float4v{acc[u / 4][u % 4 * 4], acc[u / 4][u % 4 * 4 + 1], acc[u / 4][u % 4 * 4 + 2], acc[u / 4][u % 4 * 4 + 3]};
+    for (int d = 0; d < NDT; ++d) acc[d] = zero;
+    constexpr int GP = 8 / NDT;                              // parts under way together
+    for (int p0 = 0; p0 < nparts; p0 += GP) {
+      float4v v[GP][4 * NDT];
+      float2 w[GP];
+#pragma unroll
+      for (int g = 0; g < GP; ++g) {
+        const int p = min(p0 + g, nparts - 1);
+        w[g] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, p * PER + ml, 0, 16));
+#pragma unroll
+        for (int u = 0; u < 4 * NDT; ++u) v[g][u] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(rs, p * PER + tid * 16 + u * 4096, 0, 16));
       }
-      const float x = __builtin_amdgcn_exp2f(w.x - top);
-      all = fmaf(x, w.y, all);
 #pragma unroll
-      for (int u = 0; u < 4 * NDT; ++u)
+      for (int g = 0; g < GP; ++g) {
+        if (p0 + g >= nparts) break;
+        const float x = __builtin_amdgcn_exp2f(w[g].x - top);
+        all = fmaf(x, w[g].y, all);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) total[u / 4][u % 4 * 4 + j] = fmaf(x, v[u][j], total[u / 4][u % 4 * 4 + j]);
+        for (int u = 0; u < 4 * NDT; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[u / 4][u % 4 * 4 + j] = fmaf(x, v[g][u][j], acc[u / 4][u % 4 * 4 + j]);
+      }
     }
     l = all;
-#pragma unroll
-    for (int d = 0; d < NDT; ++d) acc[d] = total[d];
   }
   if (row < rows) {
     const int t = (r0 + row) / Gq;
@@ -735,6 +739,7 @@ extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const voi
   const bool token = (long long)max_q * (H / G) <= A8_ROWS;
   const long long blocks = token ? 1 : ((long long)max_q * (H / G) + A8P_ROWS - 1) / A8P_ROWS, units = (long long)B * G * blocks;
   const long long per = token ? A8_ROWS * (D + 2) : A8P_ROWS * (D + 4);     // floats of a part
+  if (!token && parts > A8P_PARTS) return (int)hipErrorInvalidValue;
   if (token ? G > 65535 || B > 65535 || parts > 1 << 24 : units * parts > 1 << 30) return (int)hipErrorInvalidValue;
   if ((long long)G * blk * D >= 1LL << 31 || blocks > 1 << 24 || parts * per * 4 >= 1LL << 31)
     return (int)hipErrorInvalidValue;
