@@ -82,12 +82,13 @@ struct Linear4Args {
 };
 
 // MT: tiles of 16 rows of x; FT: tiles of features of a wave, which share its x; GS: MFMAs (of 32 columns) a group. A block's
-// codes, scales and zeros are asked for while the block before is worked on, and the x of one tile of rows.
+// codes, scales and zeros are asked for while the block before is worked on, and the x of up to two tiles of rows.
 template <int MT, int FT, int GS, bool Z> struct L4Block {
   static constexpr int NG = 4 / GS;
+  static constexpr bool SHARE = !Z && MT <= 2;     // one MFMA of -136 for all features (with four tiles of rows its registers cost more)
   l4_u4 c[FT];
   unsigned s[FT][2 * NG], z[FT];
-  bf16x8 x[MT == 1 ? 4 : 1];
+  bf16x8 x[MT <= 2 ? MT : 1][4];
 };
 
 // a wave-uniform address and a lane's offset, as the loads take them (64-bit sums a lane were a tenth of the loop)
@@ -99,6 +100,7 @@ template <int MT, int FT, int GS, bool Z, int NW>
 __global__ __launch_bounds__(NW * 64) void linear4_kernel(Linear4Args A) {
   using Block = L4Block<MT, FT, GS, Z>;
   constexpr int NG = Block::NG;
+  constexpr bool SHARE = Block::SHARE;
   __shared__ float4v sums[NW][FT][MT][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, fq = lane >> 4;
   const int tiles = (A.N + L4_TILE - 1) / L4_TILE, tile0 = blockIdx.x * FT, m0 = blockIdx.y * (16 * MT);
@@ -135,9 +137,11 @@ __global__ __launch_bounds__(NW * 64) void linear4_kernel(Linear4Args A) {
       if constexpr (Z && NG == 2) b.z[f] = l4_at<unsigned short>(A.zeros + at * 32, li * 2);
       if constexpr (Z && NG == 4) b.z[f] = l4_at<unsigned>(A.zeros + at * 64, li * 4);
     }
-    if constexpr (MT == 1) {
+    if constexpr (MT <= 2) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) b.x[s] = xread(0, kb, s);
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) b.x[t][s] = xread(t, kb, s);
     }
   };
   auto work = [&](const Block& b, int kb) __attribute__((always_inline)) {
@@ -146,17 +150,24 @@ __global__ __launch_bounds__(NW * 64) void linear4_kernel(Linear4Args A) {
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        if constexpr (MT == 1) x[t][s] = b.x[s];
+        if constexpr (MT <= 2) x[t][s] = b.x[t][s];
         else x[t][s] = xread(t, kb, s);
       }
-    float4v part[FT][MT];
+    float4v part[FT][MT], less[MT];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       if (kb * L4_K + 32 * s >= A.K) break;       // uniform
       const int g = s / GS;
+      constexpr unsigned M136 = 0xc308c308u;      // -136
+      if constexpr (SHARE) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          less[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, l4_u4{M136, M136, M136, M136}), x[t][s],
+                                                            s % GS == 0 ? zero : less[t], 0, 0, 0);
+      }
 #pragma unroll
       for (int f = 0; f < FT; ++f) {
-        l4_u4 w, minus = {0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};      // -136
+        l4_u4 w, minus = {M136, M136, M136, M136};
         if constexpr (Z) {
           const unsigned z = (b.z[f] >> (8 * g)) & 255u, m = z | z << 16 | 0xc300c300u;
           minus = l4_u4{m, m, m, m};
@@ -165,8 +176,9 @@ __global__ __launch_bounds__(NW * 64) void linear4_kernel(Linear4Args A) {
         for (int p = 0; p < 4; ++p) w[p] = ((b.c[f][s] >> (4 * p)) & 0x000f000fu) | magic;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          part[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, minus), x[t][s], s % GS == 0 ? zero : part[f][t], 0, 0, 0);
-          part[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), x[t][s], part[f][t], 0, 0, 0);
+          if constexpr (!SHARE)
+            part[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, minus), x[t][s], s % GS == 0 ? zero : part[f][t], 0, 0, 0);
+          part[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), x[t][s], SHARE && s % GS == 0 ? zero : part[f][t], 0, 0, 0);
         }
         if (s % GS == GS - 1) {
           const unsigned s0 = b.s[f][2 * g], s1 = b.s[f][2 * g + 1];
@@ -174,7 +186,7 @@ __global__ __launch_bounds__(NW * 64) void linear4_kernel(Linear4Args A) {
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[f][t][j] = fmaf(scale[j], part[f][t][j], acc[f][t][j]);
+            for (int j = 0; j < 4; ++j) acc[f][t][j] = fmaf(scale[j], SHARE ? part[f][t][j] + less[t][0] : part[f][t][j], acc[f][t][j]);   // less: all rows alike
         }
       }
     }
@@ -230,10 +242,10 @@ template <int MT, int FT, int GS, int NW> static void l4_go(const Linear4Args& a
 // way; of one, there are four times as many workgroups. us by (tiles a wave, waves), cold weights, launches in a replayed graph:
 // 1 row x 28672 x 4096 (groups of 128) 20.8 (1, 8), 17.1 (2, 8), 16.6 (4, 8), 15.0 (4, 4); 8 rows (64, zeros) 28.2, 20.8, 19.9, 17.0;
 // 4 x 12288 x 4096 11.6, 10.8, 9.8, 9.5; 4 x 8192 x 4096 7.7, 6.3, 8.4, 9.0; 1 x 4096 x 4096 4.4, 5.3, 7.4, 7.7; 32 rows x 14336 x
-// 4096 36.1, 21.7, 15.8, 20.5; 64 rows 64.2, 37.3, 23.4, 27.6, x 4096 x 4096 17.7, 18.5, 20.8, 25.8.
+// 4096 39.8, 23.4, 15.5, 14.0; 64 rows 64.2, 37.3, 23.4, 27.6, x 4096 x 4096 17.7, 18.5, 20.8, 25.8.
 template <int MT, int GS> static void l4_features(const Linear4Args& a, hipStream_t st) {
   const int tiles = (a.N + L4_TILE - 1) / L4_TILE;
-  if (tiles >= 640) return l4_go<MT, 4, GS, MT == 1 ? 4 : 8>(a, st);
+  if (tiles >= 640) return l4_go<MT, 4, GS, MT <= 2 ? 4 : 8>(a, st);
   if (tiles >= 384) return l4_go<MT, 2, GS, 8>(a, st);
   l4_go<MT, 1, GS, 8>(a, st);
 }
