@@ -169,7 +169,7 @@ extern "C" int loqa_rope_append8(const void* qkv, long ld, const void* cs, int c
 
 // ------------------------------------------------------------------ rows back
 // Row cu[b] + i of the results is position first[b] + i of sequence b, in bf16 (code * scale, rounded once);
-// zeros from a page that does not exist. A thread has eight entries of keys and of values.
+// zeros from a page that does not exist and in rows of no sequence. A thread has eight entries of keys and of values.
 struct Read8Args {
   const unsigned char *k, *v;
   const float *ks, *vs;
@@ -191,9 +191,9 @@ __global__ __launch_bounds__(256) void read8_kernel(Read8Args A) {
     if (A.cu[mid] <= t) lo = mid;
     else hi = mid;
   }
-  if (t < A.cu[lo] || t >= A.cu[lo + 1]) return;  // rows of no sequence stay as they are
+  const bool in = t >= A.cu[lo] && t < A.cu[lo + 1];
   const int pos = A.first[lo] + t - A.cu[lo];
-  const int pj = pos >> A.sh, page = pos < 0 || pj >= A.max_blocks ? -1 : A.bt[(size_t)lo * A.max_blocks + pj];
+  const int pj = pos >> A.sh, page = !in || pos < 0 || pj >= A.max_blocks ? -1 : A.bt[(size_t)lo * A.max_blocks + pj];
   uint4 ko = make_uint4(0, 0, 0, 0), vo = ko;
   if ((unsigned)page < (unsigned)A.n_blocks) {
     const size_t at = (size_t)page * A.G + g, off = ((at << A.sh) + (pos & ((1 << A.sh) - 1))) * D + c * 8;

@@ -242,6 +242,8 @@ bool rows_on(const at::Tensor& t, long cols, const at::Device& dev) {
   return t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.size(1) >= cols && (t.stride(1) == 1 || t.size(1) == 1) &&
          (t.size(0) <= 1 || t.stride(0) >= cols) && t.device() == dev;
 }
+// what a row's stride is where there is a second row, and one that any launch takes where there is none
+long row_stride(const at::Tensor& t) { return t.size(0) > 1 ? (long)t.stride(0) : (long)((t.size(1) + 7) / 8 * 8); }
 at::Tensor made(at::IntArrayRef size, at::ScalarType type, const at::Device& dev) {
   return at::empty(size, at::TensorOptions().dtype(type).device(dev));
 }
@@ -258,7 +260,7 @@ PyObject* cache8_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const long T = x.size(0), B = t[3]->numel();
     if (T == 0 || B == 0 || t[2]->numel() != B + 1 || bt.dim() != 2 || bt.size(0) != B || bt.size(1) == 0) Py_RETURN_NONE;
     const at::Tensor y = t[1] ? *t[1] : made({T, v[1]}, at::kBFloat16, dev);
-    return Py_BuildValue("lllllNl", T, B, (long)bt.size(1), (long)x.stride(0), (long)y.stride(0), THPVariable_Wrap(y), (long)dev.index());
+    return Py_BuildValue("lllllNl", T, B, (long)bt.size(1), row_stride(x), row_stride(y), THPVariable_Wrap(y), (long)dev.index());
   });
 }
 
@@ -284,11 +286,11 @@ PyObject* rope_append8(PyObject*, PyObject* const* args, Py_ssize_t n) {
                  !t[5]->is_contiguous() || t[5]->device() != dev || ((size_t)t[5]->data_ptr() & 15)))
       Py_RETURN_NONE;
     const at::Tensor q = t[1] ? *t[1] : made({T, H * D}, at::kBFloat16, dev);
-    if ((((size_t)x.data_ptr() | (size_t)q.data_ptr()) & 7) || ((x.stride(0) | q.stride(0)) & 3)) Py_RETURN_NONE;
+    if ((((size_t)x.data_ptr() | (size_t)q.data_ptr()) & 7) || ((row_stride(x) | row_stride(q)) & 3)) Py_RETURN_NONE;
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = loqa_rope_append8(x.data_ptr(), x.stride(0), t[5] ? t[5]->data_ptr() : nullptr, t[5] ? (int)t[5]->size(0) : 0, t[6]->data_ptr(), t[7]->data_ptr(),
-                           t[8]->data_ptr(), t[9]->data_ptr(), t[2]->data_ptr(), t[3]->data_ptr(), bt.data_ptr(), q.data_ptr(), q.stride(0), (int)T,
+    rc = loqa_rope_append8(x.data_ptr(), row_stride(x), t[5] ? t[5]->data_ptr() : nullptr, t[5] ? (int)t[5]->size(0) : 0, t[6]->data_ptr(), t[7]->data_ptr(),
+                           t[8]->data_ptr(), t[9]->data_ptr(), t[2]->data_ptr(), t[3]->data_ptr(), bt.data_ptr(), q.data_ptr(), row_stride(q), (int)T,
                            (int)B, (int)H, (int)G, (int)D, (int)v[3], (int)v[4], (int)bt.size(1), (int)std::min(v[5], T), (int)v[6], (stream_t)v[8]);
     Py_END_ALLOW_THREADS
     return rc ? launched(rc, "rope_append8") : THPVariable_Wrap(q);
@@ -359,11 +361,11 @@ PyObject* linear4_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Device dev = t[1]->device();
     const long N = v[0], K = v[1];
     if (x.scalar_type() != at::kBFloat16 || x.device() != dev || x.dim() != 2 || x.size(1) != K || x.size(0) == 0 || x.stride(1) != 1 ||
-        x.stride(0) < 0 || x.stride(0) % 8 || ((size_t)x.data_ptr() & 15))
+        row_stride(x) < 0 || row_stride(x) % 8 || ((size_t)x.data_ptr() & 15))
       Py_RETURN_NONE;
     if (t[2] && (t[2]->scalar_type() != at::kBFloat16 || t[2]->dim() != 1 || t[2]->size(0) != N || !t[2]->is_contiguous() || t[2]->device() != dev))
       Py_RETURN_NONE;
-    return Py_BuildValue("llNl", (long)x.size(0), (long)x.stride(0), THPVariable_Wrap(made({x.size(0), N}, at::kBFloat16, dev)), (long)dev.index());
+    return Py_BuildValue("llNl", (long)x.size(0), row_stride(x), THPVariable_Wrap(made({x.size(0), N}, at::kBFloat16, dev)), (long)dev.index());
   });
 }
 

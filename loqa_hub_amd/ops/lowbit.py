@@ -95,7 +95,8 @@ class Cache8:
         _need(self.n_blocks > 0 and self.n_kv > 0, "a cache without pages")
         _need(self.head_dim in HEAD_DIMS, f"head_dim is one of {HEAD_DIMS}, got {self.head_dim}")
         _need(self.block_size >= 16 and self.block_size & (self.block_size - 1) == 0, "block_size is a power of two from 16 on")
-        _need(self.n_blocks * self.block_size < 1 << 31, "slots of 32 bits")
+        _need(self.n_blocks * self.block_size < 1 << 31 and self.n_kv * self.block_size * self.head_dim < 1 << 31,
+              "slots and places within a page have 32 bits")
 
     @classmethod
     def empty(cls, n_blocks: int, n_kv: int, block_size: int, head_dim: int, dtype=torch.int8, device=None) -> "Cache8":
@@ -142,7 +143,7 @@ def rope_append8(qkv: torch.Tensor, cos_sin: torch.Tensor | None, cache: Cache8,
 
     qkv: [T, >= (H + 2 Hkv) * D] bf16, q | k | v; cos_sin: [max_pos, D/2, 2] f32 or None (no rotation), which covers every
     position (rows past its end are turned by its last entry). ``max_q`` bounds the rows of a sequence. Rotated keys
-    go to their codes without a rounding in between. Rows at positions below zero or past the block table are not
+    go to their codes without a rounding in between (qkv whose rows do not start at 8 bytes is copied first). Rows at positions below zero or past the block table are not
     appended. An infinite or NaN entry makes its page's scale so, and with it what attention gives for the page."""
     if cache.cuda:
         dev = torch._C._cuda_getDevice()
@@ -167,7 +168,12 @@ def rope_append8(qkv: torch.Tensor, cos_sin: torch.Tensor | None, cache: Cache8,
         return q_out
     if not cache.cuda:
         return ref.rope_append8(qkv, cos_sin, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, q_out=q_out)
-    _need((qkv.data_ptr() | q_out.data_ptr()) % 8 == 0 and (qkv.stride(0) | q_out.stride(0)) % 4 == 0, "rows of qkv and q_out must start at 8 bytes")
+    _need(q_out.data_ptr() % 8 == 0 and (T == 1 or q_out.stride(0) % 4 == 0), "rows of q_out must start at 8 bytes")
+    if qkv.data_ptr() % 8 or (T > 1 and qkv.stride(0) % 4):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+        if qkv.stride(0) % 4:
+            qkv = torch.nn.functional.pad(qkv, (0, -qkv.shape[1] % 4))
+        return rope_append8(qkv, cos_sin, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, q_out=q_out)
     return _elsewhere(cache, rope_append8, qkv, cos_sin, cache, cu_q, ctx_lens, block_tables, n_heads=H, max_q=max_q, q_out=q_out)
 
 

@@ -144,6 +144,13 @@ def test_append_kernel_is_the_reference(feeds, pasts, H, G, D, page, dtype, rope
     _same(dev, cache)
     lowbit.rope_append8(there[0], there[1], dev, *there[2:], n_heads=H, max_q=max(feeds))        # the same rows again change nothing
     _same(dev, cache)
+    # rows at odd places, of an odd width
+    odd = torch.empty(qkv.shape[0], qkv.shape[1] + 1, dtype=BF16, device="cuda")[:, 1:]
+    odd.copy_(qkv)
+    again = lowbit.rope_append8(odd, there[1], dev, *there[2:], n_heads=H, max_q=max(feeds))
+    rows = sum(feeds)
+    assert torch.equal(again[:rows].cpu(), b[:rows, :H * D])
+    _same(dev, cache)
 
 
 @KINDS
@@ -231,9 +238,12 @@ def test_read(dtype, dev, D, P):
                 want[at + i, 0] = cpu.k[p, :, pos % P].float().to(F64) * cpu.k_scale[p].to(F64)[:, None]
                 want[at + i, 1] = cpu.v[p, :, pos % P].float().to(F64) * cpu.v_scale[p].to(F64)[:, None]
         at += n
-    k, v = lowbit.read8(_to(cpu, dev), _cu(ns, dev), _i(first, dev), bt.to(dev), total=sum(ns))
+    k, v = lowbit.read8(_to(cpu, dev), _cu(ns, dev), _i(first, dev), bt.to(dev), total=sum(ns) + 3)
     for got, w in ((k, want[:, 0]), (v, want[:, 1])):
-        assert ((got.cpu().to(F64) - w).abs() <= (2.0 ** -8 + 2.0 ** -23) * w.abs()).all()
+        assert ((got[:-3].cpu().to(F64) - w).abs() <= (2.0 ** -8 + 2.0 ** -23) * w.abs()).all() and (got[-3:] == 0).all()
+    for total in (0, 5):
+        none = lowbit.read8(_to(cpu, dev), _i([0], dev), _i([], dev), torch.zeros(0, 4, dtype=I32, device=dev), total=total)
+        assert all(t.shape == (total, G, D) and (t == 0).all() for t in none)
 
 
 # ------------------------------------------------------------------ attention
