@@ -3,9 +3,11 @@
 //
 //   x_j = q . k_j (f16 MFMAs, f32 sums),  s_j = scale log2(e) ks x_j,  o = sum_j 2^(s_j) vs v_j / sum_j 2^(s_j)
 //
-// with ks, vs of a key's page. The values' scale goes into the exponent: t_j = s_j + log2(vs), weights w_j = 2^(t_j - max t)
-// are what the codes of v are summed up with, at most one and so f16 without a range of their own (11 bits; under 2^-14
-// an absolute 2^-25), and the denominator is sum_j w_j / vs in f32. Queries enter as f16 times a power of two of
+// with ks, vs of a key's page. The values' scale goes into the exponent: t_j = s_j + log2(vs), weights w_j = 2^(t_j - m)
+// are what the codes of v are summed up with, and the denominator is sum_j w_j / vs in f32. The reference m of a row follows its
+// largest t_j within a factor of 2^8, so weights are f16 without a range of their own: 11 bits each, under 2^-14 an absolute 2^-25
+// (with a reference that never lags, some row of a wave has a new maximum in nearly every tile, and rescaling is a tenth
+// of a tile's instructions). Queries enter as f16 times a power of two of
 // the row that puts its largest entry in 2^14 .. 2^15: bf16's 8 bits are exact down to 2^-28 of it.
 //
 // Rows that see no key (a position before the first) give zeros; keys of pages that do not exist count as masked.
@@ -88,8 +90,8 @@ __device__ __forceinline__ int a8_lift(float top) {
   return top > 0.f && top < INFINITY ? min(14 - (int)((__float_as_uint(top) >> 23) & 255) + 127, 126) : 0;
 }
 
-// ---- the partials of a row block's parts, joined by the last of them. R rows; a thread's accumulators are put at
-// (row, column), four columns a piece. Written through and read past the caches: parts may run on different XCDs.
+// ---- the partials of a unit's parts, joined by the last of them: [unit][part][R rows][D columns, then maximum and sum]. Written
+// through and read past the caches: parts may run on different XCDs.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t a8_rsrc(const Attn8Args& A, size_t unit, int part, int rows, int D) {
   return __builtin_amdgcn_make_buffer_rsrc(A.ws + (unit * A.parts + part) * rows * (D + 2), 0, rows * (D + 2) * 4, 0x00020000);
 }
@@ -166,7 +168,11 @@ __device__ __forceinline__ void a8_join(const Attn8Args& A, size_t unit, int n, 
 // Up to 16 rows per kv head. A step reads every cached code once, so it is bound by the bytes a compute unit has
 // under way: each wave streams tiles of 32 keys straight to its own ring of two in LDS, as the bf16 form does
 // (attn_stream.hip), the scales of a tile's two pages with it. The waves of a workgroup take tiles in turn, the
-// workgroups of a sequence parts of its keys.
+// workgroups of a sequence parts of its keys. A tile is 8 KB to the bf16 form's 16 and as much work: page numbers are scalars
+// that no wait precedes (kept in an array they went through LDS, and a tile waited for the next one's: 32 x 4000 keys x 8
+// heads of 128 66 us), values are asked of LDS ahead of the exponentials. us, cold caches, pages of 16 (bf16 form): 32 x 4000 keys x 8
+// heads of 128 52 (96), 4.8 TB/s; 1 x 100000 47, 4.4; 256 x 1000 90 (159); 8 x 600 10 (13); 1 x 600 6.9 (10.9); 64 x 300 13 (21); 8 x
+// 1500 x 20 of 64 13 (19).
 //
 //   S^T = K Q^T   : 16 x 16 x 32 MFMAs; a lane reads 16 codes of a key at once, the K slots of two MFMAs
 //   O^T += V^T P^T: eight keys of one column by a transposing read of bytes; P^T is the accumulator as it stands
@@ -420,7 +426,15 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
 // ------------------------------------------------------------------ prompts
 // 128 rows a workgroup, 32 a wave, over tiles of 64 keys: the workgroup fetches a tile's codes to registers while it works
 // on the tile before, widens them to f16 rows in LDS (two stages), and computes S^T = K Q^T and O^T += V^T P^T with
-// 32 x 32 x 16 MFMAs as the bf16 form does (flash_pipe.h: layouts and swizzles).
+// 32 x 32 x 16 MFMAs as the bf16 form does (flash_pipe.h: layouts and swizzles). Widening rides between the scores' MFMAs, a
+// group's exponentials between the MFMAs of the group before.
+// What bounds it is the issue of vector instructions: at 128 columns a tile of a wave has 350 of them, 32 exponentials
+// among them, 64 to 128 to widen its share of the codes, beside 32 MFMAs (1024 cycles) and 60 LDS accesses: 3700 cycles alone on
+// its SIMD, 5100 for two waves that share it. 2048 causal rows x 32 query heads over 8 of 128 columns 58 us (0.59 PFLOP/s; the bf16 form,
+// whose keys and values go to LDS as they are, 56), 1024 32, 512 17; 3 x 113 rows behind 5000 keys, 64 columns, 34.
+// Taken back: pages and addresses on the scalar unit (fewer vector instructions, but a chain of scalar ones in their place: 58 -> 66 us);
+// the longest parts first, counted by a lane for each block (2048 rows 79); six and eight fragments of K in flight, halves of a chunk
+// swapped against bank conflicts of the writes (nothing).
 #define A8P_ROWS 128
 #define A8P_KEYS 64
 #define A8P_PARTS 16

