@@ -122,21 +122,24 @@ __device__ __forceinline__ void a8_put(bf16_t* at, const float4v& o, float l, bo
   }
 }
 
-// joins n parts of `rows` rows in order and writes them; NT threads, eight partials under way
+// Joins n parts of `rows` rows and writes them; NT threads, eight partials under way each. A thread has four columns of a row, and
+// where there are threads left (few rows), as many of them share the parts as there are whole groups: they meet in LDS
+// (at `room`, NT * 24 bytes), in order. (Two contexts of 27000 keys x 2 heads of 64 in 120 parts
+// each 23.6 -> 15.4 us.)
 template <int D, int R, int NT, typename Put>
-__device__ __forceinline__ void a8_join(const Attn8Args& A, size_t unit, int n, int rows, Put&& put) {
+__device__ __forceinline__ void a8_join(const Attn8Args& A, size_t unit, int n, int rows, float* room, Put&& put) {
   constexpr int OB = 8, PER = R * (D + 2) * 4;
   const auto rs = __builtin_amdgcn_make_buffer_rsrc(A.ws + unit * A.parts * R * (D + 2), 0, A.parts * PER, 0x00020000);
-  for (int id = threadIdx.x; id < rows * (D / 4); id += NT) {
-    const int r = id / (D / 4), c = id % (D / 4) * 4;
-    float ms = A8_NONE, l = 0.f;
-    float4v o = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < n; s0 += OB) {
+  auto sum = [&](int r, int c, int from, int to, float& ms, float& l, float4v& o) __attribute__((always_inline)) {
+    ms = A8_NONE;
+    l = 0.f;
+    o = float4v{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = from; s0 < to; s0 += OB) {
       float4v v[OB];
       float2 ml[OB];
 #pragma unroll
       for (int i = 0; i < OB; ++i) {
-        const int at = min(s0 + i, n - 1) * PER;
+        const int at = min(s0 + i, to - 1) * PER;
         ml[i] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, at + (R * D + 2 * r) * 4, 0, 16));
         v[i] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(rs, at + (r * D + c) * 4, 0, 16));
       }
@@ -153,15 +156,43 @@ __device__ __forceinline__ void a8_join(const Attn8Args& A, size_t unit, int n, 
       for (int j = 0; j < 4; ++j) o[j] *= a;
 #pragma unroll
       for (int i = 0; i < OB; ++i) {
-        if (s0 + i >= n) break;
+        if (s0 + i >= to) break;
         const float x = exp2f(ml[i].x - ms);
         l += x * ml[i].y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] += x * v[i][j];
       }
     }
-    put(r, c, o, l);
+  };
+  const int items = rows * (D / 4), groups = n > OB ? max(1, min(NT / items, (n + OB - 1) / OB)) : 1;
+  float ms, l;
+  float4v o;
+  if (groups == 1) {
+    for (int id = threadIdx.x; id < items; id += NT) {
+      sum(id / (D / 4), id % (D / 4) * 4, 0, n, ms, l, o);
+      put(id / (D / 4), id % (D / 4) * 4, o, l);
+    }
+    return;
   }
+  const int g = threadIdx.x / items, id = threadIdx.x - g * items, r = id / (D / 4), c = id % (D / 4) * 4;
+  if (g < groups) {
+    sum(r, c, n * g / groups, n * (g + 1) / groups, ms, l, o);
+    float* at = room + threadIdx.x * 6;
+    at[0] = ms; at[1] = l;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) at[2 + j] = o[j];
+  }
+  __syncthreads();
+  if (g > 0) return;
+  for (int k = 1; k < groups; ++k) {
+    const float* at = room + (k * items + id) * 6;
+    const float mn = fmaxf(ms, at[0]), a = exp2f(ms - mn), x = exp2f(at[0] - mn);
+    ms = mn;
+    l = l * a + at[1] * x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = o[j] * a + at[2 + j] * x;
+  }
+  put(r, c, o, l);
 }
 
 // ------------------------------------------------------------------ token steps
@@ -420,7 +451,7 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
   }
   if (nparts == 1) return;
   if (!a8_last(A.tickets + unit * TICKET, nparts, reinterpret_cast<int*>(lds + L::MERGE - 16))) return;
-  a8_join<D, A8_ROWS, A8_WAVES * 64>(A, unit, nparts, rows, put);
+  a8_join<D, A8_ROWS, A8_WAVES * 64>(A, unit, nparts, rows, reinterpret_cast<float*>(lds), put);
 }
 
 // ------------------------------------------------------------------ prompts

@@ -242,10 +242,11 @@ template <int MT, int FT, int GS, int NW> static void l4_go(const Linear4Args& a
 // way; of one, there are four times as many workgroups. us by (tiles a wave, waves), cold weights, launches in a replayed graph:
 // 1 row x 28672 x 4096 (groups of 128) 20.8 (1, 8), 17.1 (2, 8), 16.6 (4, 8), 15.0 (4, 4); 8 rows (64, zeros) 28.2, 20.8, 19.9, 17.0;
 // 4 x 12288 x 4096 11.6, 10.8, 9.8, 9.5; 4 x 8192 x 4096 7.7, 6.3, 8.4, 9.0; 1 x 4096 x 4096 4.4, 5.3, 7.4, 7.7; 32 rows x 14336 x
-// 4096 39.8, 23.4, 15.5, 14.0; 64 rows 64.2, 37.3, 23.4, 27.6, x 4096 x 4096 17.7, 18.5, 20.8, 25.8.
+// 4096 39.8, 23.4, 15.5, 14.0; 64 rows 64.2, 37.3, 23.4, 27.6, x 4096 x 4096 17.7, 18.5, 20.8, 25.8; 18 rows x 8656 x
+// 8448 38.2, 29.9, 21.2, 19.8, 32 x 4096 x 4096 11.9, 12.3, 13.9, 12.8.
 template <int MT, int GS> static void l4_features(const Linear4Args& a, hipStream_t st) {
   const int tiles = (a.N + L4_TILE - 1) / L4_TILE;
-  if (tiles >= 640) return l4_go<MT, 4, GS, MT <= 2 ? 4 : 8>(a, st);
+  if (tiles >= (MT == 2 ? 384 : 640)) return l4_go<MT, 4, GS, MT <= 2 ? 4 : 8>(a, st);
   if (tiles >= 384) return l4_go<MT, 2, GS, 8>(a, st);
   l4_go<MT, 1, GS, 8>(a, st);
 }

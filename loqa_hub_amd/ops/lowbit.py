@@ -202,8 +202,10 @@ def attn8_plan(max_q: int, group: int, units: int, keys: int, D: int) -> tuple[i
     if max_q * group <= TOKEN_ROWS:
         # a workgroup for each compute unit, two of 64 columns, and no part of less than a tile for each wave. us by parts: 1 context of
         # 100000 x 8 heads of 128 86 (12), 53.5 (24), 47.6 (32), 53.9 (48), 56.3 (64); 32 of 4000 52.4 (1), 53.9 (2), 57.3 (4); 8 of
-        # 600 10.6 (1), 9.9 (5); 1 of 4000 41.1 (1), 12.1 (8), 11.3 (16, 32); 8 of 1500 x 20 of 64 15.4 (1), 13.3 (3), 14.2 (6)
-        parts = max(1, min(round(TOKEN_SLOTS[D] / units), -(-keys // 128)))
+        # 600 10.6 (1), 9.9 (5); 1 of 4000 41.1 (1), 12.1 (8), 11.3 (16, 32); 8 of 1500 x 20 of 64 15.4 (1), 13.3
+        # (3), 14.2 (6); more than 48 cost their join more than they bring: 2 of 26690 x 2 of 64 15.7 (24), 13.4 (48), 13.0 (64), 15.4
+        # (128); 1 of 20000 x 1 of 128 15.0 (32), 14.6 (48), 19.9 (157)
+        parts = max(1, min(round(TOKEN_SLOTS[D] / units), -(-keys // 128), 48))
         return (parts, 1 if keys <= 128 * parts else 2, *((units * parts * TOKEN_ROWS * (D + 2), units) if parts > 1 else (0, 0)))
     blocks, most = -(-max_q * group // PROMPT_ROWS), max(1, -(-keys // 64))
     parts = max(1, min(PROMPT_SLOTS[D] // (units * blocks), most // 4, 16))
