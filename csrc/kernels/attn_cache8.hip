@@ -459,10 +459,11 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
 // on the tile before, widens them to f16 rows in LDS (two stages), and computes S^T = K Q^T and O^T += V^T P^T with
 // 32 x 32 x 16 MFMAs as the bf16 form does (flash_pipe.h: layouts and swizzles). Widening rides between the scores' MFMAs, a
 // group's exponentials between the MFMAs of the group before.
-// What bounds it is the issue of vector instructions: at 128 columns a tile of a wave has 350 of them, 32 exponentials
-// among them, 64 to 128 to widen its share of the codes, beside 32 MFMAs (1024 cycles) and 60 LDS accesses: 3700 cycles alone on
-// its SIMD, 5100 for two waves that share it. 2048 causal rows x 32 query heads over 8 of 128 columns 58 us (0.59 PFLOP/s; the bf16 form,
-// whose keys and values go to LDS as they are, 56), 1024 32, 512 17; 3 x 113 rows behind 5000 keys, 64 columns, 34.
+// What bounds it: at 128 columns two waves share a SIMD (registers, and 64 KB of stages), and of 2400 cycles that a tile of one takes
+// there its vector instructions have 1500 (310 of them, 32 exponentials among them, 40 to 90 to widen its share of the codes),
+// its 32 MFMAs 1024, LDS a third; the rest is waiting for each other, at the barrier and behind the scores.
+// 2048 causal rows x 32 query heads over 8 of 128 columns 56 us (0.61 PFLOP/s; the bf16 form,
+// whose keys and values go to LDS as they are, 56), 1024 31, 512 17; 3 x 113 rows behind 5000 keys, 64 columns, 34.
 // Taken back: pages and addresses on the scalar unit (fewer vector instructions, but a chain of scalar ones in their place: 58 -> 66 us);
 // the longest parts first, counted by a lane for each block (2048 rows 79); six and eight fragments of K in flight, halves of a chunk
 // swapped against bank conflicts of the writes (nothing).
@@ -472,7 +473,6 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
 
 template <int D> struct A8Prompt {
   static constexpr int K = A8P_KEYS * D * 2, STAGE = 2 * K;
-  static_assert((STAGE & (STAGE - 1)) == 0, "stages differ in one bit of an address, the array starts at a multiple of both");
   static constexpr int SCALES = 2 * STAGE, SMEM = 2 * STAGE + 2 * 64;    // [stage][ks 4, log2 vs 4, 1 / vs 4]
 };
 
@@ -481,7 +481,7 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   using L = A8Prompt<D>;
   constexpr int NS = D / 16, NDT = D / 32, CH = D / 16, N = A8P_KEYS * CH / 256;    // chunks of 16 codes a row, a thread
   static_assert(N * 256 == A8P_KEYS * CH, "whole chunks a thread");
-  __shared__ __attribute__((aligned(2 * L::STAGE))) unsigned char lds[L::SMEM];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[L::SMEM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, li = lane & 15;
   // (sequence, kv head) from the workgroup's number modulo as many, so that a head's workgroups share an XCD's L2 where these are a
   // multiple of eight
@@ -521,8 +521,9 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     for (int i = 0; i < N; ++i) pages[i] = bt[(unsigned)min(kt + cr + i * (256 / CH), last) >> A.sh];
     group_page = bt[(unsigned)min(kt + 16 * (tid & 3), last) >> A.sh];
   };
-  auto fetch = [&](int kt) __attribute__((always_inline)) {
-    bool none = kt + A8P_KEYS > last + 1;
+  bool none = false;
+  auto ask = [&](int kt) __attribute__((always_inline)) {
+    none = kt + A8P_KEYS > last + 1;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const unsigned key = min(kt + cr + i * (256 / CH), last), page = (unsigned)pages[i] < (unsigned)A.n_blocks ? pages[i] : 0;
@@ -531,6 +532,8 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
       vw[i] = *reinterpret_cast<const uint4*>(at + to_v);
       none |= page != (unsigned)pages[i];
     }
+  };
+  auto asked = [&](int kt) __attribute__((always_inline)) {    // what of it branches, and the pages of the tile behind
     if (__any(none)) {                                       // codes that are none may be NaN, which no weight of zero hides
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -542,6 +545,7 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
       sk = A.ks[at];
       sv = A.vs[at];
     }
+    look(kt + A8P_KEYS);
   };
   // piece q of the tile in registers: 8 codes, of keys or of values, widened and put where the fragments are read from
   constexpr int PIECES = 4 * N;
@@ -551,9 +555,9 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     const int sw = q & 2 ? fl_vswz<D>(cr) : fl_kswz<D>(cr);
     put_at[q] = base + (q & 2 ? L::K : 0) + cr * (D * 2) + ((2 * cc + (q & 1)) ^ sw) * 16;
   }
-  auto store = [&](int q) __attribute__((always_inline)) {
+  auto store = [&](int stage, int q) __attribute__((always_inline)) {
     const uint4 w = q & 2 ? vw[q >> 2] : kw[q >> 2];
-    *fl_lds<c8_h8>(put_at[q & 3] + (q >> 2) * (256 / CH) * D * 2) = q & 1 ? c8_widen8<KIND>(w.z, w.w) : c8_widen8<KIND>(w.x, w.y);
+    *fl_lds<c8_h8>(put_at[q & 3] + stage * L::STAGE + (q >> 2) * (256 / CH) * D * 2) = q & 1 ? c8_widen8<KIND>(w.z, w.w) : c8_widen8<KIND>(w.x, w.y);
   };
   static_assert(256 / CH % 16 == 0, "a thread's rows share a swizzle");
   auto store_scales = [&](int stage) __attribute__((always_inline)) {
@@ -594,61 +598,100 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
 
   if (n > 0) {
     const int kt = i0 * A8P_KEYS;
-    fetch(kt);
-    look(kt + A8P_KEYS);
+    ask(kt);
+    asked(kt);
 #pragma unroll
-    for (int q = 0; q < PIECES; ++q) store(q);
+    for (int q = 0; q < PIECES; ++q) store(0, q);
     store_scales(0);
-    fetch(kt + A8P_KEYS);
-    look(kt + 2 * A8P_KEYS);
+    ask(kt + A8P_KEYS);
+    asked(kt + A8P_KEYS);
   }
+  // A tile: the scores of its first 32 keys, beside which the next tile is widened; those of the second 32 beside the weights of the
+  // first, to the reference as it stands; the maxima, which move it where they have to (then the weights are taken once more); the
+  // values' products of the first 32 keys beside the weights of the second; those of the second beside the addresses of the tile after
+  // the next. (One after the other, stages toggled in registers: the 2048 rows above 58 us, 56 now.)
   constexpr int KR = 4, VR = 4;                              // fragments in flight + 1
   // rows of this wave that some key of a tile from here on is hidden from, or that end in it
   const int edge = min(f.keys, A.causal ? f.past + (r0 + wave * 32) / Gq + 1 : f.keys) - A8P_KEYS;
-  for (int i = 0; i < n; ++i) {
-    const int stage = i & 1, kt = (i0 + i) * A8P_KEYS;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) put_at[q] ^= L::STAGE;       // the other stage
+  auto tile = [&](auto slot, int i) __attribute__((always_inline)) {
+    constexpr int stage = decltype(slot)::value;
+    const int kt = (i0 + i) * A8P_KEYS;
     fl_meet();                                               // this stage is written, nobody reads the other one any more; loads stay under way
     const float* sc = reinterpret_cast<const float*>(lds + L::SCALES + stage * 64);
+    const float4v ks = *reinterpret_cast<const float4v*>(sc), lv = *reinterpret_cast<const float4v*>(sc + 4), inv = *reinterpret_cast<const float4v*>(sc + 8);
     float16v s[2];
-    c8_h8 kf[KR];
-    auto kread = [&](int u) __attribute__((always_inline)) { kf[u % KR] = *fl_lds<c8_h8>(kb[u >> 1] + 32 * (u & 1) * D * 2); };
+    c8_h8 kf[KR], vf[VR], p[4];
+    float sum[4], c[4], top[4];
+    auto kread = [&](int u) __attribute__((always_inline)) { kf[u % KR] = *fl_lds<c8_h8>(kb[u % NS] + (stage * L::STAGE + 32 * (u / NS) * D * 2)); };
+    auto vread = [&](int v) __attribute__((always_inline)) {
+      const unsigned a = vb[v % NDT] + (stage * L::STAGE + 16 * (v / NDT) * D * 2);
+      const fl_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a));
+      const fl_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a + 8 * D * 2));
+      short8 a8;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { a8[j] = lo[j]; a8[4 + j] = hi[j]; }
+      vf[v % VR] = __builtin_bit_cast(c8_h8, a8);
+    };
+    auto hide = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (kt + 32 * t + (j & 3) + 8 * (j >> 2) + 4 * h > seen) s[t][j] = -INFINITY;
+    };
+    // scores j of group g (16 keys of a page): 2^(x c + log2 vs - m)
+    auto weights = [&](int g, int j0, int j1) __attribute__((always_inline)) {
+      const float off = lv[g] - m;
+#pragma unroll
+      for (int j = j0; j < j1; j += 2) {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        const f2 e = {__builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j], c[g], off)),
+                      __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j + 1], c[g], off))};
+        const c8_h2 w = __builtin_convertvector(e, c8_h2);
+        sum[g] = j == 0 ? e[0] + e[1] : sum[g] + (e[0] + e[1]);    // in f32: a weight that f16 has as zero still counts for a page of small values
+        p[g][j] = w[0];
+        p[g][j + 1] = w[1];
+      }
+    };
+    auto tops = [&](int g, int j0, int j1) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = j0; j < j1; j += 2)
+        top[g] = j == 0 ? fmaxf(s[g >> 1][8 * (g & 1)], s[g >> 1][8 * (g & 1) + 1])
+                        : fmaxf(fmaxf(top[g], s[g >> 1][8 * (g & 1) + j]), s[g >> 1][8 * (g & 1) + j + 1]);
+    };
 #pragma unroll
     for (int u = 0; u < KR - 1; ++u) kread(u);
-    // the next tile is widened between the MFMAs of this one's scores
 #pragma unroll
-    for (int u = 0; u < 2 * NS; ++u) {
-      s[u & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[u % KR], qf[u >> 1], u < 2 ? zero : s[u & 1], 0, 0, 0);
-      if (u + KR - 1 < 2 * NS) kread(u + KR - 1);
-      if (u % 2) store(u / 2);
+    for (int u = 0; u < NS; ++u) {
+      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[u % KR], qf[u], u == 0 ? zero : s[0], 0, 0, 0);
+      kread(u + KR - 1);
+      store(1 - stage, u);
       __builtin_amdgcn_sched_barrier(0);
     }
-    static_assert(PIECES == NS, "a piece every other MFMA");
-    store_scales(1 - stage);
-    fetch(kt + 2 * A8P_KEYS);
-    look(kt + 3 * A8P_KEYS);
-    if (kt > edge) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int key = kt + 32 * t + (j & 3) + 8 * (j >> 2) + 4 * h;
-          if (key > seen) s[t][j] = -INFINITY;
-        }
-    }
-    // t = x c + log2 vs with c above zero: the largest product of a group of 16 keys is its largest score
-    const float4v ks = *reinterpret_cast<const float4v*>(sc), lv = *reinterpret_cast<const float4v*>(sc + 4), inv = *reinterpret_cast<const float4v*>(sc + 8);
-    float c[4], mx = -INFINITY;
+    static_assert(PIECES == NS && KR - 1 <= NS, "a piece for every MFMA");
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const float k = factor * ks[g];
       c[g] = k < 1.1754943508222875e-38f ? 1.1754943508222875e-38f : k;     // of no use to a masked -infinity if zero; NaN stays
-      float x = s[g >> 1][8 * (g & 1)];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) x = fmaxf(x, s[g >> 1][8 * (g & 1) + j]);
-      mx = fmaxf(mx, fmaf(x, c[g], lv[g]));
     }
+    if (kt > edge) hide(0);
+    constexpr int SW = 16 / NS;                              // scores a step
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[(NS + u) % KR], qf[u], u == 0 ? zero : s[1], 0, 0, 0);
+      if (u + KR - 1 < NS) kread(NS + u + KR - 1);
+      weights(u * SW / 8, u * SW % 8, u * SW % 8 + SW);
+      tops(u * SW / 8, u * SW % 8, u * SW % 8 + SW);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    store_scales(1 - stage);
+#pragma unroll
+    for (int v = 0; v < VR - 1; ++v) vread(v);
+    if (kt > edge) hide(1);
+    tops(2, 0, 8);
+    tops(3, 0, 8);
+    // x c + log2 vs with c above zero: the largest product of a group is its largest score
+    float mx = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) mx = fmaxf(mx, fmaf(top[g], c[g], lv[g]));
     // the reference stays where it is while no row's maximum passes it by more than a factor of 2^8: f16 weights keep their 11
     // bits up to 2^15, and a prompt's first tiles nearly always raise some row of the wave
     mx = fl_max32(mx);
@@ -660,50 +703,31 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
       for (int d = 0; d < NDT; ++d)
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[d][j] *= alpha;
+      weights(0, 0, 8);
+      weights(1, 0, 8);
     }
-    // the weights of a group of keys between the MFMAs of the group before
-    c8_h8 p[2], vf[VR];
-    auto vread = [&](int v) __attribute__((always_inline)) {
-      const unsigned a = vb[v % NDT] + 16 * (v / NDT) * D * 2;
-      const fl_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a));
-      const fl_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(fl_lds<fl_v4s>(a + 8 * D * 2));
-      short8 a8;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { a8[j] = lo[j]; a8[4 + j] = hi[j]; }
-      vf[v % VR] = __builtin_bit_cast(c8_h8, a8);
-    };
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    auto weights = [&](int g, int j0, int j1) __attribute__((always_inline)) {
-      const float off = lv[g] - m;
-#pragma unroll
-      for (int j = j0; j < j1; j += 2) {
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        const f2 e = {__builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j], c[g], off)),
-                      __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j + 1], c[g], off))};
-        const c8_h2 w = __builtin_convertvector(e, c8_h2);
-        sum[g] += e[0] + e[1];                               // in f32: a weight that f16 has as zero still counts for a page of small values
-        p[g & 1][j] = w[0];
-        p[g & 1][j + 1] = w[1];
-      }
-    };
-#pragma unroll
-    for (int v = 0; v < VR - 1; ++v) vread(v);
-    weights(0, 0, 8);
     __builtin_amdgcn_sched_barrier(0);
+    constexpr int PW = 16 / (2 * NDT);
 #pragma unroll
-    for (int v = 0; v < 4 * NDT; ++v) {
-      const int g = v / NDT, d = v % NDT;
-      acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[v % VR], p[g & 1], acc[d], 0, 0, 0);
-      if (v + VR - 1 < 4 * NDT) vread(v + VR - 1);
-      if (g < 3) weights(g + 1, d * 8 / NDT, (d + 1) * 8 / NDT);
+    for (int v = 0; v < 2 * NDT; ++v) {
+      acc[v % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[v % VR], p[v / NDT], acc[v % NDT], 0, 0, 0);
+      vread(v + VR - 1);
+      weights(2 + v * PW / 8, v * PW % 8, v * PW % 8 + PW);
       __builtin_amdgcn_sched_barrier(0);
+    }
+    ask(kt + 2 * A8P_KEYS);
+#pragma unroll
+    for (int v = 2 * NDT; v < 4 * NDT; ++v) {
+      acc[v % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[v % VR], p[v / NDT], acc[v % NDT], 0, 0, 0);
+      if (v + VR - 1 < 4 * NDT) vread(v + VR - 1);
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) l = fmaf(sum[g], inv[g], l);
-#pragma unroll
-    for (int u = 0; u < NS; ++u) kb[u] ^= L::STAGE;
-#pragma unroll
-    for (int d = 0; d < NDT; ++d) vb[d] ^= L::STAGE;
+    asked(kt + 2 * A8P_KEYS);
+  };
+  for (int i = 0; i < n; i += 2) {                           // a stage's places are constants of its copy of the code
+    tile(Fl<0>{}, i);
+    if (i + 1 < n) tile(Fl<1>{}, i + 1);
   }
   l = fl_both32(l);                                          // a lane has summed up its half of the keys
   const size_t unit = ((size_t)b * A.G + kvh) * A.row_blocks + block;
