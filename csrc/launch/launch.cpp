@@ -56,7 +56,8 @@ int loqa_attention8(const void*, long, const void*, const void*, const void*, co
                     int, int, int, int, int, int, int, int, int, float, int, int, int, int, void*, long, void*, long, stream_t);
 int loqa_page_step(const void*, const void*, void*, void*, const void*, void*, void*, void*, void*, void*, void*, void*, void*, int, int, int,
                    int, int, stream_t);
-int loqa_linear4(const void*, long, const void*, const void*, const void*, const void*, void*, long, int, int, int, int, stream_t);
+int loqa_linear4(const void*, long, const void*, const void*, const void*, const void*, void*, long, int, int, int, int, int, int, void*, long, void*,
+                 long, stream_t);
 }
 
 namespace {
@@ -353,19 +354,29 @@ PyObject* page_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// (x, the weight's codes, bias or None; N, K) -> (rows, row stride, y [rows of x.., N], device)
+// (x, codes, scales, zeros or None, bias or None; N, K, group, current device, its stream) -> y of up to 16 rows on the current
+// device, as a whole call; otherwise (rows, row stride, y to fill, device)
 PyObject* linear4_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  return checked<3, 2>(args, n, [](const at::Tensor* const* t, const long* v) -> PyObject* {
-    if (!t[0] || !t[1] || !t[1]->is_cuda()) Py_RETURN_NONE;
+  return checked<5, 5>(args, n, [](const at::Tensor* const* t, const long* v) -> PyObject* {
+    if (!t[0] || !t[1] || !t[2] || !t[1]->is_cuda()) Py_RETURN_NONE;
     const at::Tensor& x = *t[0];
     const at::Device dev = t[1]->device();
     const long N = v[0], K = v[1];
     if (x.scalar_type() != at::kBFloat16 || x.device() != dev || x.dim() != 2 || x.size(1) != K || x.size(0) == 0 || x.stride(1) != 1 ||
         row_stride(x) < 0 || row_stride(x) % 8 || ((size_t)x.data_ptr() & 15))
       Py_RETURN_NONE;
-    if (t[2] && (t[2]->scalar_type() != at::kBFloat16 || t[2]->dim() != 1 || t[2]->size(0) != N || !t[2]->is_contiguous() || t[2]->device() != dev))
+    if (t[4] && (t[4]->scalar_type() != at::kBFloat16 || t[4]->dim() != 1 || t[4]->size(0) != N || !t[4]->is_contiguous() || t[4]->device() != dev))
       Py_RETURN_NONE;
-    return Py_BuildValue("llNl", (long)x.size(0), row_stride(x), THPVariable_Wrap(made({x.size(0), N}, at::kBFloat16, dev)), (long)dev.index());
+    const at::Tensor y = made({x.size(0), N}, at::kBFloat16, dev);
+    if (x.size(0) > 16 || dev.index() != v[3])
+      return Py_BuildValue("llNl", (long)x.size(0), row_stride(x), THPVariable_Wrap(y), (long)dev.index());
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = loqa_linear4(x.data_ptr(), row_stride(x), t[1]->data_ptr(), t[2]->data_ptr(), t[3] ? t[3]->data_ptr() : nullptr,
+                      t[4] ? t[4]->data_ptr() : nullptr, y.data_ptr(), N, (int)x.size(0), (int)N, (int)K, (int)v[2], 0, 1, nullptr, 0, nullptr, 0,
+                      (stream_t)v[4]);
+    Py_END_ALLOW_THREADS
+    return rc ? launched(rc, "linear4") : THPVariable_Wrap(y);
   });
 }
 

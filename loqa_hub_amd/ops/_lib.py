@@ -300,7 +300,7 @@ _LOWBIT_SIGS = {
                         _l, _vp],
     "loqa_page_step": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
     "loqa_shuffle4": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
-    "loqa_linear4": [_vp, _l, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _vp],
+    "loqa_linear4": [_vp, _l, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _i, _vp, _l, _vp, _l, _vp],
 }
 _lowbit = None
 

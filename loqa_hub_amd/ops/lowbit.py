@@ -377,10 +377,36 @@ class Weight4:
         return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zeros) if t is not None)
 
 
+@functools.lru_cache(maxsize=4096)
+def linear4_plan(M: int, N: int, K: int) -> tuple[int, int, int, int]:
+    """(tiles of 16 features a wave of the kernel for more rows, or 0: the one for few rows; parts of K; floats of workspace,
+    tickets) of a product of M rows with an [N, K] weight."""
+    # us, few rows' kernel and the other, cold weights: 32 x 512 x 8192 17.3, 7.3; 32 x 4096 x 14336 30.8, 14; 32 x 28672 x 4096
+    # 29.7, 24; 24 x 10240 x 2048 9.7, 8.6; 18 x 4096 x 4096 9.0, 8.0; 24 x 2048 x 2048 6.2, 5.9; 20 x 4096 x 2048 5.9, 6.5; 32 x 256 x
+    # 512 3.4, 5.0
+    if M <= 16 or (M <= 32 and K <= 2048 and N <= 4096):
+        return 0, 1, 0, 0
+    # one and two tiles a wave: 64 x 28672 x 4096 42, 37, 32 rows 25.2, 24; 64 x 24368 x 2144 20.6, 20.6; 40 x 16384 x 2048 13.1, 15.2; 17 x
+    # 8192 x 4096 10.4, 11.5; 64 x 4096 x 4096 10.6, 13
+    features = 2 if N >= 24576 else 1
+    # two workgroups for each compute unit, and no part of less than two blocks of 128 columns: 64 x 4096 x 4096 22.4 (1), 11.1
+    # (4), 10.6 (8), 15.4 (16); 20 x 3584 x 13696 47 (1), 17 (4), 13.5 (9), 14.8 (16); 64 x 14336 x 4096 24.5 (1), 20.0 (2), 23 (4)
+    rows, blocks = 32 if M <= 32 else 64, -(-K // 128)
+    units = -(-N // (64 * features)) * -(-M // rows)
+    parts = max(1, min(512 // units, blocks // 2, 16))
+    parts = -(-blocks // -(-blocks // parts))
+    return (features, parts, units * parts * 64 * features * rows, units) if parts > 1 else (features, 1, 0, 0)
+
+
 def linear4(x: torch.Tensor, w: Weight4, b: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] bf16 times the transpose of a 4-bit weight (+ bias [N] bf16): [..., N] bf16, summed up in f32. Made for
     the few rows of token steps; more than 64 read the weight again for every 64. An infinite or NaN entry of x makes its row NaN."""
-    fast = kernels().linear4_rows(x, w.codes, b, w.n, w.k) if w.cuda else None
+    fast = None
+    if w.cuda:
+        dev = torch._C._cuda_getDevice()
+        fast = kernels().linear4_rows(x, w.codes, w.scales, w.zeros, b, w.n, w.k, w.group, dev, _stream(dev))
+        if type(fast) is torch.Tensor:
+            return fast
     if fast is None:
         _typed(x, torch.bfloat16, "x")
         _need(x.dim() >= 1 and x.shape[-1] == w.k, f"x has {w.k} columns")
@@ -395,6 +421,10 @@ def linear4(x: torch.Tensor, w: Weight4, b: torch.Tensor | None = None) -> torch
         rows = x.reshape(-1, w.k).clone(memory_format=torch.contiguous_format)     # whole rows at 16 bytes
         return linear4(rows, w, b).view(*x.shape[:-1], w.n)
     M, ld, y, dev = fast
+    features, parts, floats, tiles = linear4_plan(M, w.n, w.k)
+    st = _stream(dev)
     with _there(dev):
-        check(kernels().loqa_linear4(x, ld, w.codes, w.scales, w.zeros, b, y, w.n, M, w.n, w.k, w.group, _stream(dev)), "linear4")
+        ws, tickets = _sk_workspace(x.device, st, floats, tiles) if parts > 1 else (None, None)
+        check(kernels().loqa_linear4(x, ld, w.codes, w.scales, w.zeros, b, y, w.n, M, w.n, w.k, w.group, features, parts, ws,
+                                     0 if ws is None else ws.numel(), tickets, 0 if tickets is None else tickets.numel(), st), "linear4")
     return y

@@ -477,6 +477,58 @@ def test_linear4(M, N, K, group, zeros, bias, dev):
     assert lowbit.linear4(x.to(dev)[:0], w4).shape == (0, N)
 
 
+@pytest.mark.parametrize("M,N,K,group,zeros", [(17, 200, 4224, 32, True), (32, 4104, 96, 32, False), (24, 40, 2176, 128, True), (33, 24600, 160, 32, True), (64, 24576, 512, 128, False),
+                                               (40, 70, 5184, 64, True), (100, 333, 1152, 64, False), (20, 24592, 288, 32, True), (32, 64, 2112, 64, False)])
+@pytest.mark.parametrize("dev", DEVICES)
+def test_linear4_more_rows(M, N, K, group, zeros, dev):
+    """Rows that share x in LDS: parts of K, ends inside a block, a tile and a workgroup's tiles, and what lies around y stays."""
+    g = torch.Generator().manual_seed(M + N + K)
+    codes = torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, generator=g)
+    scales = (0.02 * torch.randn(N, K // group, generator=g)).to(BF16)
+    z = torch.randint(0, 16, (N, K // group), dtype=torch.uint8, generator=g) if zeros else None
+    x, b = torch.randn(M, K, generator=g).to(BF16), torch.randn(N, generator=g).to(BF16)
+    w = ref.dense4(codes, scales, z).to(F64)
+    w4 = lowbit.Weight4(codes.to(dev), scales.to(dev), z.to(dev) if zeros else None)
+    y = x.to(F64) @ w.t() + b.to(F64)
+    got = lowbit.linear4(x.to(dev), w4, b.to(dev))
+    assert got.shape == (M, N) and ((got.cpu().to(F64) - y).abs() <= oracle.linear4_bound(y, x, w, scales)).all()
+    for _ in range(3):
+        assert torch.equal(lowbit.linear4(x.to(dev), w4, b.to(dev)), got)
+    # a row that is no number stays the only one
+    x[M // 2, K - 1] = math.inf
+    odd = lowbit.linear4(x.to(dev), w4, b.to(dev))
+    rows = torch.arange(M, device=dev) != M // 2
+    assert torch.equal(odd[rows], got[rows]) and not odd[~rows].isfinite().any()
+
+
+@pytest.mark.gpu
+def test_linear4_parts_in_graphs_and_streams():
+    """Products in parts of K: a captured one replayed between eager ones, and two streams at once."""
+    g = torch.Generator("cuda").manual_seed(3)
+    ws = [lowbit.Weight4(*(t.cuda() for t in lowbit.quantize4(torch.randn(n, k, generator=torch.Generator().manual_seed(n)), 64, True))) for n, k in
+          ((320, 4096), (700, 2304))]
+    x = [torch.randn(48, w.k, device="cuda", generator=g).to(BF16) for w in ws]
+    graph = torch.cuda.CUDAGraph()
+    for a, w in zip(x, ws):
+        lowbit.linear4(a, w)
+    with ops.graph_capture(graph):
+        out = [lowbit.linear4(a, w) for a, w in zip(x, ws)]
+    streams = [torch.cuda.Stream() for _ in ws]
+    for i in range(5):
+        for a in x:
+            a.normal_(generator=g)
+        want = [lowbit.linear4(a, w) for a, w in zip(x, ws)]
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+        torch.cuda.synchronize()
+        got = []
+        for st, a, w in zip(streams, x, ws):
+            with torch.cuda.stream(st):
+                got.append([lowbit.linear4(a, w) for _ in range(4)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, b) for ys, b in zip(got, want) for y in ys), i
+
+
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_quantize4(zeros, group):
