@@ -207,7 +207,7 @@ __device__ __forceinline__ void a8_join(const Attn8Args& A, size_t unit, int n, 
 //
 //   S^T = K Q^T   : 16 x 16 x 32 MFMAs; a lane reads 16 codes of a key at once, the K slots of two MFMAs
 //   O^T += V^T P^T: eight keys of one column by a transposing read of bytes; P^T is the accumulator as it stands
-#define A8_ROWS 16
+#define A8_ROWS 32                     // at most
 #define A8_TILE 32
 #define A8_WAVES 4
 #define A8_LDS __attribute__((address_space(3)))
@@ -230,10 +230,11 @@ __device__ __forceinline__ a8_u4 a8_raw(const unsigned char* base, unsigned byte
 template <int N> __device__ __forceinline__ void a8_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // R: stages of a wave's ring; one where no wave has a second tile, so that twice as many workgroups fit a compute unit
-template <int D, int R> struct A8Token {
+template <int D, int R, int RT> struct A8Token {
+  static constexpr int ROWS = 16 * RT;
   static constexpr int TB = A8_TILE * D, STAGE = 2 * TB + 256;         // K, V, a dword a lane of scales
   static constexpr int RING = R * STAGE;
-  static constexpr int MERGE = A8_WAVES * A8_ROWS * (D + 4 + 2) * 4 + 16;
+  static constexpr int MERGE = A8_WAVES * ROWS * (D + 4 + 2) * 4 + 16;
   static constexpr int SMEM = A8_WAVES * RING > MERGE ? A8_WAVES * RING : MERGE;
   static constexpr int FIT = 163840 / SMEM < 4 ? 163840 / SMEM : 4;    // workgroups of a compute unit
 };
@@ -248,9 +249,10 @@ __device__ __forceinline__ float a8_sum16(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-template <int D, int KIND, int R>
-__global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_token_kernel(Attn8Args A) {
-  using L = A8Token<D, R>;
+template <int D, int KIND, int R, int RT>
+__global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R, RT>::FIT)) void attn8_token_kernel(Attn8Args A) {
+  using L = A8Token<D, R, RT>;
+  constexpr int ROWS = L::ROWS;
   constexpr int LPR = D / 16, RPL = 64 / LPR, NL = A8_TILE / RPL;      // lanes a row, rows a load, loads of K (and of V)
   constexpr int NS = D / 64, ND = D / 16, LD = D + 4;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[L::SMEM];
@@ -269,16 +271,18 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
   // page numbers of the tile asked for next and of the one behind it
   int pa0 = page_at(kt0), pa1 = page_at(kt0 + 16), pb0 = R > 1 ? page_at(kt0 + STEP) : 0, pb1 = R > 1 ? page_at(kt0 + STEP + 16) : 0;
 
-  // the queries of row li, asked for ahead of the first tile: K slots (fq, e) of MFMAs 2 s and 2 s + 1 are columns 64 s + 16 fq + e
+  // the queries of rows 16 r + li, asked for ahead of the first tile: K slots (fq, e) of MFMAs 2 s and 2 s + 1 are columns 64 s + 16 fq + e
   // and + 8 + e
-  const int tok = li / Gq;
-  const bool row = li < rows;
-  uint4 x[2 * NS];
-  {
-    const bf16_t* qp = A.q + (size_t)(f.q0 + (row ? tok : 0)) * A.ldq + (size_t)(kvh * Gq + (row ? li - tok * Gq : 0)) * D + 16 * fq;
-    a8_row(A, x, [&](int u) { return qp + u / 2 * 64 + u % 2 * 8; });
+  uint4 x[RT][2 * NS];
+  int seen[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int at = 16 * r + li, tok = at / Gq;
+    const bool row = at < rows;
+    const bf16_t* qp = A.q + (size_t)(f.q0 + (row ? tok : 0)) * A.ldq + (size_t)(kvh * Gq + (row ? at - tok * Gq : 0)) * D + 16 * fq;
+    a8_row(A, x[r], [&](int u) { return qp + u / 2 * 64 + u % 2 * 8; });
+    seen[r] = min(A.causal ? f.past + tok : 0x7fffffff, kend - 1);
   }
-  const int qpos = A.causal ? f.past + tok : 0x7fffffff, seen = min(qpos, kend - 1);
 
   // chunk (16 codes) c of row r lies at place c ^ swz(r)
   auto swz = [](int row) { return D == 64 ? (row >> 1) & 3 : row & 7; };
@@ -315,12 +319,13 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
   if constexpr (R > 1) ask(kt0 + STEP, ring + L::STAGE, pb0, pb1);
 
   // (waits for the rows, and with them for the tiles behind, which the compiler does not count)
-  c8_h8 qf[2 * NS];
-  float factor;
-  {
-    const int e = a8_lift(a8_max16(fl_max32(a8_top(x))));
-    factor = ldexpf(A.scale_log2, -e);
-    a8_queries(x, row, e, false, qf);
+  c8_h8 qf[RT][2 * NS];
+  float factor[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int e = a8_lift(a8_max16(fl_max32(a8_top(x[r]))));
+    factor[r] = ldexpf(A.scale_log2, -e);
+    a8_queries(x[r], 16 * r + li < rows, e, false, qf[r]);
   }
   unsigned kat[NS], vat[ND];                     // places of the fragments in a stage
 #pragma unroll
@@ -331,10 +336,15 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
     const int r = 16 * (li >> 3) + 4 * fq + ((li >> 1) & 3);
     vat[d] = ring + L::TB + r * D + ((d ^ swz(r)) * 16) + (li & 1) * 8;
   }
-  float4v acc[ND];
+  float4v acc[RT][ND];
+  float m_run[RT], l_run[RT];
 #pragma unroll
-  for (int d = 0; d < ND; ++d) acc[d] = float4v{0.f, 0.f, 0.f, 0.f};
-  float m_run = A8_NONE, l_run = 0.f;
+  for (int r = 0; r < RT; ++r) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[r][d] = float4v{0.f, 0.f, 0.f, 0.f};
+    m_run[r] = A8_NONE;
+    l_run[r] = 0.f;
+  }
   unsigned slot = 0;
   for (int kt = kt0; kt < kend; kt += STEP) {
     int next0 = 0, next1 = 0;                    // wanted behind this tile's work
@@ -347,54 +357,74 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
     a8_v2i vw[ND];                               // asked for here, wanted behind the exponentials
 #pragma unroll
     for (int d = 0; d < ND; ++d) vw[d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(a8_lds<a8_v2i>(vat[d] + slot));
-    float4v st[2] = {float4v{0.f, 0.f, 0.f, 0.f}, float4v{0.f, 0.f, 0.f, 0.f}};
+    float4v st[RT][2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) st[r][0] = st[r][1] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < 2 * NS; ++u) {
-      st[u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c8_widen8<KIND>(kw[u][0], kw[u][1]), qf[u & ~1], st[u & 1], 0, 0, 0);
-      st[u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c8_widen8<KIND>(kw[u][2], kw[u][3]), qf[u | 1], st[u & 1], 0, 0, 0);
+      const c8_h8 lo = c8_widen8<KIND>(kw[u][0], kw[u][1]), hi = c8_widen8<KIND>(kw[u][2], kw[u][3]);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) st[r][u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qf[r][u & ~1], st[r][u & 1], 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) st[r][u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qf[r][u | 1], st[r][u & 1], 0, 0, 0);
     }
-    float mx = -INFINITY, inv[2];
+    float ks[2], lv[2], inv[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const bool there = (unsigned)(t ? pa1 : pa0) < (unsigned)A.n_blocks;
-      const float vs = a8_least(sc[2 + t]), c = there ? factor * a8_least(sc[t]) : 0.f, lv = there ? __builtin_amdgcn_logf(vs) : -INFINITY;
+      const float vs = a8_least(sc[2 + t]);
+      ks[t] = there ? a8_least(sc[t]) : 0.f;
+      lv[t] = there ? __builtin_amdgcn_logf(vs) : -INFINITY;
       inv[t] = there ? __builtin_amdgcn_rcpf(vs) : 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) st[t][j] = fmaf(st[t][j], c, lv);
     }
-    if (kt + A8_TILE > kend || (A.causal && kt + A8_TILE - 1 > f.past)) {
+    const bool edge = kt + A8_TILE > kend || (A.causal && kt + A8_TILE - 1 > f.past);
+    c8_h8 p[RT];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int r = 0; r < RT; ++r) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (kt + 16 * t + 4 * fq + j > seen) st[t][j] = -INFINITY;
-    }
+      for (int t = 0; t < 2; ++t) {
+        const float c = factor[r] * ks[t];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, st[j >> 2][j & 3]);
-    mx = a8_max16(fl_max32(mx));
-    if (__any(mx > m_run + 8.f)) {               // as in the prompt form
-      const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-      m_run = m_new;
-      l_run *= alpha;
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[d][j] *= alpha;
-    }
-    c8_h8 p;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = __builtin_amdgcn_exp2f(st[t][j] - m_run);
-        sum += e;
-        p[4 * t + j] = (_Float16)e;
+        for (int j = 0; j < 4; ++j) st[r][t][j] = fmaf(st[r][t][j], c, lv[t]);
       }
-      l_run = fmaf(sum, inv[t], l_run);          // of this lane's keys
+      if (edge) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (kt + 16 * t + 4 * fq + j > seen[r]) st[r][t][j] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mx = fmaxf(mx, st[r][j >> 2][j & 3]);
+      mx = a8_max16(fl_max32(mx));
+      if (__any(mx > m_run[r] + 8.f)) {          // as in the prompt form
+        const float m_new = fmaxf(m_run[r], mx), alpha = __builtin_amdgcn_exp2f(m_run[r] - m_new);
+        m_run[r] = m_new;
+        l_run[r] *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[r][d][j] *= alpha;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float e = __builtin_amdgcn_exp2f(st[r][t][j] - m_run[r]);
+          sum += e;
+          p[r][4 * t + j] = (_Float16)e;
+        }
+        l_run[r] = fmaf(sum, inv[t], l_run[r]);  // of this lane's keys
+      }
     }
 #pragma unroll
-    for (int d = 0; d < ND; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c8_widen8<KIND>(vw[d][0], vw[d][1]), p, acc[d], 0, 0, 0);
+    for (int d = 0; d < ND; ++d) {
+      const c8_h8 w = c8_widen8<KIND>(vw[d][0], vw[d][1]);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) acc[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, p[r], acc[r][d], 0, 0, 0);
+    }
     if constexpr (R > 1) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot has been read
       ask(kt + 2 * STEP, ring + slot, next0, next1);
@@ -407,16 +437,19 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
     }
   }
   a8_wait<0>();                                  // no load into LDS outlives the loop
-  l_run = a8_sum16(fl_both32(l_run));
   __syncthreads();
   float* so = reinterpret_cast<float*>(lds);             // [wave][row][LD]
-  float* sm = so + A8_WAVES * A8_ROWS * LD;              // [wave][m, l][row]
-  if (li < rows) {
+  float* sm = so + A8_WAVES * ROWS * LD;                 // [wave][m, l][row]
 #pragma unroll
-    for (int d = 0; d < ND; ++d) *reinterpret_cast<float4v*>(so + (wave * A8_ROWS + li) * LD + 16 * d + 4 * fq) = acc[d];
+  for (int r = 0; r < RT; ++r) {
+    const int at = 16 * r + li;
+    const float l = a8_sum16(fl_both32(l_run[r]));
+    if (at >= rows) continue;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) *reinterpret_cast<float4v*>(so + (wave * ROWS + at) * LD + 16 * d + 4 * fq) = acc[r][d];
     if (fq == 0) {
-      sm[(2 * wave) * A8_ROWS + li] = m_run;
-      sm[(2 * wave + 1) * A8_ROWS + li] = l_run;
+      sm[(2 * wave) * ROWS + at] = m_run[r];
+      sm[(2 * wave + 1) * ROWS + at] = l;
     }
   }
   __syncthreads();
@@ -426,19 +459,19 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
     const int t = r / Gq;
     a8_put(A.out + (size_t)(f.q0 + t) * A.ldo + (size_t)(kvh * Gq + r - t * Gq) * D + c, o, l, whole);
   };
-  const auto rs = a8_rsrc(A, nparts > 1 ? unit : 0, nparts > 1 ? part : 0, A8_ROWS, D);
+  const auto rs = a8_rsrc(A, nparts > 1 ? unit : 0, nparts > 1 ? part : 0, ROWS, D);
   for (int id = tid; id < rows * (D / 4); id += A8_WAVES * 64) {
     const int r = id / (D / 4), c = id % (D / 4) * 4;
     float ms = sm[r];
 #pragma unroll
-    for (int w = 1; w < A8_WAVES; ++w) ms = fmaxf(ms, sm[2 * w * A8_ROWS + r]);
+    for (int w = 1; w < A8_WAVES; ++w) ms = fmaxf(ms, sm[2 * w * ROWS + r]);
     float l = 0.f;
     float4v o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < A8_WAVES; ++w) {
-      const float x = exp2f(sm[2 * w * A8_ROWS + r] - ms);
-      l += sm[(2 * w + 1) * A8_ROWS + r] * x;
-      const float4v v = *reinterpret_cast<const float4v*>(so + (w * A8_ROWS + r) * LD + c);
+      const float x = exp2f(sm[2 * w * ROWS + r] - ms);
+      l += sm[(2 * w + 1) * ROWS + r] * x;
+      const float4v v = *reinterpret_cast<const float4v*>(so + (w * ROWS + r) * LD + c);
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] += x * v[j];
     }
@@ -446,12 +479,12 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R>::FIT)) void attn8_tok
       put(r, c, o, l);
     } else {
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(a8_u4, o), rs, (r * D + c) * 4, 0, 16);
-      if (c == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(a8_u2, make_float2(ms, l)), rs, (A8_ROWS * D + 2 * r) * 4, 0, 16);
+      if (c == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(a8_u2, make_float2(ms, l)), rs, (ROWS * D + 2 * r) * 4, 0, 16);
     }
   }
   if (nparts == 1) return;
   if (!a8_last(A.tickets + unit * TICKET, nparts, reinterpret_cast<int*>(lds + L::MERGE - 16))) return;
-  a8_join<D, A8_ROWS, A8_WAVES * 64>(A, unit, nparts, rows, reinterpret_cast<float*>(lds), put);
+  a8_join<D, ROWS, A8_WAVES * 64>(A, unit, nparts, rows, reinterpret_cast<float*>(lds), put);
 }
 
 // ------------------------------------------------------------------ prompts
@@ -805,9 +838,9 @@ extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const voi
   if ((D != 64 && D != 128) || (kind != C8_INT8 && kind != C8_E4M3) || blk < 16 || (blk & (blk - 1)) || G <= 0 || H <= 0 || H % G ||
       n_blocks <= 0 || max_blocks <= 0 || parts <= 0 || each <= 0)
     return (int)hipErrorInvalidValue;
-  const bool token = (long long)max_q * (H / G) <= A8_ROWS;
+  const bool token = (long long)max_q * (H / G) <= A8_ROWS, two = token && max_q * (H / G) > 16;
   const long long blocks = token ? 1 : ((long long)max_q * (H / G) + A8P_ROWS - 1) / A8P_ROWS, units = (long long)B * G * blocks;
-  const long long per = token ? A8_ROWS * (D + 2) : A8P_ROWS * (D + 4);     // floats of a part
+  const long long per = token ? (two ? 32 : 16) * (D + 2) : A8P_ROWS * (D + 4);     // floats of a part
   if (!token && parts > A8P_PARTS) return (int)hipErrorInvalidValue;
   if (token ? G > 65535 || B > 65535 || parts > 1 << 24 : units * parts > 1 << 30) return (int)hipErrorInvalidValue;
   if ((long long)G * blk * D >= 1LL << 31 || blocks > 1 << 24 || parts * per * 4 >= 1LL << 31)
@@ -818,11 +851,13 @@ extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const voi
                     max_q, parts, causal, (int)blocks, each, parts == 1 && units <= 512, scale * 1.4426950408889634f};
   if (token) {
     const dim3 grid(parts, G, B);
-#define GO(D_, K_) do { if (each == 1) hipLaunchKernelGGL((attn8_token_kernel<D_, K_, 1>), grid, dim3(A8_WAVES * 64), 0, st, a); \
-                        else hipLaunchKernelGGL((attn8_token_kernel<D_, K_, 2>), grid, dim3(A8_WAVES * 64), 0, st, a); } while (0)
+#define GO1(D_, K_, R_, RT_) hipLaunchKernelGGL((attn8_token_kernel<D_, K_, R_, RT_>), grid, dim3(A8_WAVES * 64), 0, st, a)
+#define GO(D_, K_) do { if (two) { if (each == 1) GO1(D_, K_, 1, 2); else GO1(D_, K_, 2, 2); } \
+                        else if (each == 1) GO1(D_, K_, 1, 1); else GO1(D_, K_, 2, 1); } while (0)
     if (D == 64) { if (kind == C8_INT8) GO(64, C8_INT8); else GO(64, C8_E4M3); }
     else { if (kind == C8_INT8) GO(128, C8_INT8); else GO(128, C8_E4M3); }
 #undef GO
+#undef GO1
   } else {
     const dim3 grid((unsigned)(units * parts));
 #define GO(D_, K_) hipLaunchKernelGGL((attn8_prompt_kernel<D_, K_>), grid, dim3(256), 0, st, a)

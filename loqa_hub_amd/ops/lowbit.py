@@ -31,8 +31,8 @@ from ._lib import check, kernels, ptr, stream_ptr
 
 CACHE_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 HEAD_DIMS = (64, 128)
-TOKEN_ROWS, PROMPT_ROWS = 16, 128     # rows of a workgroup of the two forms (csrc/kernels/attn_cache8.hip)
-TOKEN_SLOTS, PROMPT_SLOTS = {64: 512, 128: 256}, {64: 768, 128: 512}    # their workgroups at once, by head_dim
+TOKEN_ROWS, PROMPT_ROWS = 32, 128     # rows of a workgroup of the two forms (csrc/kernels/attn_cache8.hip)
+TOKEN_SLOTS, PROMPT_SLOTS = 512, {64: 768, 128: 512}    # their workgroups at once, by head_dim
 
 
 def _need(ok: bool, what: str) -> None:
@@ -200,13 +200,18 @@ def attn8_plan(max_q: int, group: int, units: int, keys: int, D: int) -> tuple[i
     """(parts of a sequence's keys at most, tiles of 64 keys of a prompt's part or stages of a token's ring, floats of workspace, tickets) for ``units``
     (sequence, kv head) pairs of up to ``max_q`` rows, ``group`` heads and ``keys`` keys."""
     if max_q * group <= TOKEN_ROWS:
-        # a workgroup for each compute unit, two of 64 columns, and no part of less than a tile for each wave. us by parts: 1 context of
-        # 100000 x 8 heads of 128 86 (12), 53.5 (24), 47.6 (32), 53.9 (48), 56.3 (64); 32 of 4000 52.4 (1), 53.9 (2), 57.3 (4); 8 of
-        # 600 10.6 (1), 9.9 (5); 1 of 4000 41.1 (1), 12.1 (8), 11.3 (16, 32); 8 of 1500 x 20 of 64 15.4 (1), 13.3
-        # (3), 14.2 (6); more than 48 cost their join more than they bring: 2 of 26690 x 2 of 64 15.7 (24), 13.4 (48), 13.0 (64), 15.4
-        # (128); 1 of 20000 x 1 of 128 15.0 (32), 14.6 (48), 19.9 (157)
-        parts = max(1, min(round(TOKEN_SLOTS[D] / units), -(-keys // 128), 48))
-        return (parts, 1 if keys <= 128 * parts else 2, *((units * parts * TOKEN_ROWS * (D + 2), units) if parts > 1 else (0, 0)))
+        # Two workgroups for each compute unit, no part of less than a tile for each wave, and, since a unit's parts are joined by one of
+        # them, about the square root of its keys. us by parts, heads of 128 (contexts x keys x kv heads): 16 x 4000 x 8 40.7 (1), 33.6
+        # (2), 35.1 (3), 31.0 (4), 35.8 (6); 12 x 4000 x 8 38.1 (1), 26.1 (2), 30.6 (3), 26.7 (4), 29.8 (6); 24 x 4000 x 8 45.4 (1), 48.8
+        # (2), 32 of them 55.5 (1), 58.4 (2); 1 x 2000 x 8 of 8 rows 20.5 (1), 11.4 (4), 9.8 (8), 9.5 (16), of 32 rows 26.2, 17.6, 15.9,
+        # 18.6; 1 x 30000 x 8 of 8 rows 25.4 (16), 22.6 (24), 22.9 (32), 25.0 (48), of 32 rows 37.0, 35.7, 37.2, 45.3; 64 columns: 1 x
+        # 20000 x 1 of 5 rows 16.2 (16), 13.3 (24), 12.7 (32), 11.9 (48); 32 x 4000 x 8 36.7 (1), 31.2 (2), 32.1 (4)
+        rows = max_q * group
+        parts, few = TOKEN_SLOTS // units, rows * D <= 1024
+        if D == 128 and parts < 3:
+            parts = 1
+        parts = max(1, min(parts, -(-keys // 128), max(math.isqrt(keys // 8), 16) if few else math.isqrt(keys // 32), 48 if D == 64 else 32))
+        return (parts, 1 if keys <= 128 * parts else 2, *((units * parts * (16 if rows <= 16 else 32) * (D + 2), units) if parts > 1 else (0, 0)))
     blocks, most = -(-max_q * group // PROMPT_ROWS), max(1, -(-keys // 64))
     parts = max(1, min(PROMPT_SLOTS[D] // (units * blocks), most // 4, 16))
     return (parts, -(-most // parts), units * blocks * parts * PROMPT_ROWS * (D + 4), units * blocks) if parts > 1 else (1, most, 0, 0)
