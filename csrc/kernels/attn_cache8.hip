@@ -207,7 +207,6 @@ __device__ __forceinline__ void a8_join(const Attn8Args& A, size_t unit, int n, 
 //
 //   S^T = K Q^T   : 16 x 16 x 32 MFMAs; a lane reads 16 codes of a key at once, the K slots of two MFMAs
 //   O^T += V^T P^T: eight keys of one column by a transposing read of bytes; P^T is the accumulator as it stands
-#define A8_ROWS 32                     // at most
 #define A8_TILE 32
 #define A8_WAVES 4
 #define A8_LDS __attribute__((address_space(3)))
@@ -502,7 +501,7 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R, RT>::FIT)) void attn8
 // swapped against bank conflicts of the writes (nothing).
 #define A8P_ROWS 128
 #define A8P_KEYS 64
-#define A8P_PARTS 16
+#define A8P_PARTS 32
 
 template <int D> struct A8Prompt {
   static constexpr int K = A8P_KEYS * D * 2, STAGE = 2 * K;
@@ -828,19 +827,20 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   }
 }
 
-// parts: of a sequence's keys at most; each: tiles of 64 keys of a prompt's part (the longer blocks have more parts); of a token step 1
+// form: 0 prompts, 1 or 2 token steps of up to 16 times as many rows; parts: of a sequence's keys at most; each: tiles of 64 keys of a prompt's part (the longer blocks have more parts); of a token step 1
 // where a wave is expected to have one tile (parts * 128 keys bound the contexts), else 2
 extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const void* v, const void* ks, const void* vs, const void* cu,
                                const void* ctx, const void* bt, void* out, long ldo, int T, int B, int H, int G, int D, int blk, int n_blocks,
-                               int max_blocks, int max_q, float scale, int causal, int kind, int parts, int each, void* ws, long ws_floats, void* tickets,
+                               int max_blocks, int max_q, float scale, int causal, int kind, int form, int parts, int each, void* ws, long ws_floats, void* tickets,
                                long n_tickets, hipStream_t st) {
   if (T <= 0 || B <= 0 || max_q <= 0) return 0;
   if ((D != 64 && D != 128) || (kind != C8_INT8 && kind != C8_E4M3) || blk < 16 || (blk & (blk - 1)) || G <= 0 || H <= 0 || H % G ||
       n_blocks <= 0 || max_blocks <= 0 || parts <= 0 || each <= 0)
     return (int)hipErrorInvalidValue;
-  const bool token = (long long)max_q * (H / G) <= A8_ROWS, two = token && max_q * (H / G) > 16;
+  const bool token = form > 0;
+  if (form < 0 || form > 2 || (token && (long long)max_q * (H / G) > 16 * form)) return (int)hipErrorInvalidValue;
   const long long blocks = token ? 1 : ((long long)max_q * (H / G) + A8P_ROWS - 1) / A8P_ROWS, units = (long long)B * G * blocks;
-  const long long per = token ? (two ? 32 : 16) * (D + 2) : A8P_ROWS * (D + 4);     // floats of a part
+  const long long per = token ? 16 * form * (D + 2) : A8P_ROWS * (D + 4);     // floats of a part
   if (!token && parts > A8P_PARTS) return (int)hipErrorInvalidValue;
   if (token ? G > 65535 || B > 65535 || parts > 1 << 24 : units * parts > 1 << 30) return (int)hipErrorInvalidValue;
   if ((long long)G * blk * D >= 1LL << 31 || blocks > 1 << 24 || parts * per * 4 >= 1LL << 31)
@@ -852,7 +852,7 @@ extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const voi
   if (token) {
     const dim3 grid(parts, G, B);
 #define GO1(D_, K_, R_, RT_) hipLaunchKernelGGL((attn8_token_kernel<D_, K_, R_, RT_>), grid, dim3(A8_WAVES * 64), 0, st, a)
-#define GO(D_, K_) do { if (two) { if (each == 1) GO1(D_, K_, 1, 2); else GO1(D_, K_, 2, 2); } \
+#define GO(D_, K_) do { if (form == 2) { if (each == 1) GO1(D_, K_, 1, 2); else GO1(D_, K_, 2, 2); } \
                         else if (each == 1) GO1(D_, K_, 1, 1); else GO1(D_, K_, 2, 1); } while (0)
     if (D == 64) { if (kind == C8_INT8) GO(64, C8_INT8); else GO(64, C8_E4M3); }
     else { if (kind == C8_INT8) GO(128, C8_INT8); else GO(128, C8_E4M3); }

@@ -53,7 +53,7 @@ int loqa_rope_append8(const void*, long, const void*, int, void*, void*, void*, 
 int loqa_read8(const void*, const void*, const void*, const void*, const void*, const void*, const void*, void*, void*, int, int, int, int, int,
                int, int, int, stream_t);
 int loqa_attention8(const void*, long, const void*, const void*, const void*, const void*, const void*, const void*, const void*, void*, long,
-                    int, int, int, int, int, int, int, int, int, float, int, int, int, int, void*, long, void*, long, stream_t);
+                    int, int, int, int, int, int, int, int, int, float, int, int, int, int, int, void*, long, void*, long, stream_t);
 int loqa_page_step(const void*, const void*, void*, void*, const void*, void*, void*, void*, void*, void*, void*, void*, void*, int, int, int,
                    int, int, stream_t);
 int loqa_linear4(const void*, long, const void*, const void*, const void*, const void*, void*, long, int, int, int, int, int, int, void*, long, void*,

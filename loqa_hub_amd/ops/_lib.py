@@ -296,7 +296,7 @@ _seqmix = None
 _LOWBIT_SIGS = {
     "loqa_rope_append8": [_vp, _l, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
     "loqa_read8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
-    "loqa_attention8": [_vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _i, _vp, _l, _vp,
+    "loqa_attention8": [_vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _i, _i, _vp, _l, _vp,
                         _l, _vp],
     "loqa_page_step": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
     "loqa_shuffle4": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],

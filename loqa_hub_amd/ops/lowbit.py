@@ -31,8 +31,8 @@ from ._lib import check, kernels, ptr, stream_ptr
 
 CACHE_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 HEAD_DIMS = (64, 128)
-TOKEN_ROWS, PROMPT_ROWS = 32, 128     # rows of a workgroup of the two forms (csrc/kernels/attn_cache8.hip)
-TOKEN_SLOTS, PROMPT_SLOTS = 512, {64: 768, 128: 512}    # their workgroups at once, by head_dim
+PROMPT_ROWS = 128                     # rows of a workgroup (csrc/kernels/attn_cache8.hip)
+SLOTS = 512                           # workgroups at once, two a compute unit
 
 
 def _need(ok: bool, what: str) -> None:
@@ -196,25 +196,42 @@ def read8(cache: Cache8, cu_k: torch.Tensor, first: torch.Tensor, block_tables: 
 
 
 @functools.lru_cache(maxsize=4096)
-def attn8_plan(max_q: int, group: int, units: int, keys: int, D: int) -> tuple[int, int, int, int]:
-    """(parts of a sequence's keys at most, tiles of 64 keys of a prompt's part or stages of a token's ring, floats of workspace, tickets) for ``units``
-    (sequence, kv head) pairs of up to ``max_q`` rows, ``group`` heads and ``keys`` keys."""
-    if max_q * group <= TOKEN_ROWS:
-        # Two workgroups for each compute unit, no part of less than a tile for each wave, and, since a unit's parts are joined by one of
-        # them, about the square root of its keys. us by parts, heads of 128 (contexts x keys x kv heads): 16 x 4000 x 8 40.7 (1), 33.6
-        # (2), 35.1 (3), 31.0 (4), 35.8 (6); 12 x 4000 x 8 38.1 (1), 26.1 (2), 30.6 (3), 26.7 (4), 29.8 (6); 24 x 4000 x 8 45.4 (1), 48.8
-        # (2), 32 of them 55.5 (1), 58.4 (2); 1 x 2000 x 8 of 8 rows 20.5 (1), 11.4 (4), 9.8 (8), 9.5 (16), of 32 rows 26.2, 17.6, 15.9,
-        # 18.6; 1 x 30000 x 8 of 8 rows 25.4 (16), 22.6 (24), 22.9 (32), 25.0 (48), of 32 rows 37.0, 35.7, 37.2, 45.3; 64 columns: 1 x
-        # 20000 x 1 of 5 rows 16.2 (16), 13.3 (24), 12.7 (32), 11.9 (48); 32 x 4000 x 8 36.7 (1), 31.2 (2), 32.1 (4)
-        rows = max_q * group
-        parts, few = TOKEN_SLOTS // units, rows * D <= 1024
-        if D == 128 and parts < 3:
-            parts = 1
-        parts = max(1, min(parts, -(-keys // 128), max(math.isqrt(keys // 8), 16) if few else math.isqrt(keys // 32), 48 if D == 64 else 32))
-        return (parts, 1 if keys <= 128 * parts else 2, *((units * parts * (16 if rows <= 16 else 32) * (D + 2), units) if parts > 1 else (0, 0)))
-    blocks, most = -(-max_q * group // PROMPT_ROWS), max(1, -(-keys // 64))
-    parts = max(1, min(PROMPT_SLOTS[D] // (units * blocks), most // 4, 16))
-    return (parts, -(-most // parts), units * blocks * parts * PROMPT_ROWS * (D + 4), units * blocks) if parts > 1 else (1, most, 0, 0)
+def attn8_plan(max_q: int, group: int, units: int, keys: int, D: int) -> tuple[int, int, int, int, int]:
+    """(form: 0 prompts, else tiles of 16 rows of a token step; parts of a sequence's keys at most; tiles of 64 keys of a prompt's part or
+    stages of a token's ring; floats of workspace; tickets) for ``units`` (sequence, kv head) pairs of up to ``max_q`` rows, ``group`` heads
+    and ``keys`` keys."""
+    rows = max_q * group
+    if rows <= 16:
+        return _token_plan(1, rows, units, keys, D)
+    if rows <= 32:
+        return _token_plan(2, rows, units, keys, D)
+    return _prompt_plan(rows, units, keys, D)
+
+
+def _token_plan(form: int, rows: int, units: int, keys: int, D: int) -> tuple[int, int, int, int, int]:
+    # Two workgroups for each compute unit, no part of less than a tile for each wave, and, since a unit's parts are joined by one of
+    # them, about the square root of its keys. us by parts, heads of 128 (contexts x keys x kv heads): 16 x 4000 x 8 40.7 (1), 33.6
+    # (2), 35.1 (3), 31.0 (4), 35.8 (6); 12 x 4000 x 8 38.1 (1), 26.1 (2), 30.6 (3), 26.7 (4), 29.8 (6); 24 x 4000 x 8 45.4 (1), 48.8
+    # (2), 32 of them 55.5 (1), 58.4 (2); 1 x 2000 x 8 of 8 rows 20.5 (1), 11.4 (4), 9.8 (8), 9.5 (16), of 32 rows 26.2, 17.6, 15.9,
+    # 18.6; 1 x 30000 x 8 of 8 rows 25.4 (16), 22.6 (24), 22.9 (32), 25.0 (48), of 32 rows 37.0, 35.7, 37.2, 45.3; 64 columns: 1 x
+    # 20000 x 1 of 5 rows 16.2 (16), 13.3 (24), 12.7 (32), 11.9 (48); 32 x 4000 x 8 36.7 (1), 31.2 (2), 32.1 (4). Many rows of few keys: 1
+    # x 300 x 8 of 32 rows 10.0 (1), 12.5 (3), 8 x 700 14.4 (1), 16.1 (4), 8 x 1500 21.8 (1), 19.9 (2), 20.4 (6)
+    parts, few = SLOTS // units, rows * D <= 1024
+    if D == 128 and parts < 3:
+        parts = 1
+    parts = max(1, min(parts, -(-keys // 128), max(math.isqrt(keys // 8), 16) if few else math.isqrt(keys // 32) if keys > 768 else 1,
+                       48 if D == 64 else 32))
+    return (form, parts, 1 if keys <= 128 * parts else 2, *((units * parts * 16 * form * (D + 2), units) if parts > 1 else (0, 0)))
+
+
+def _prompt_plan(rows: int, units: int, keys: int, D: int) -> tuple[int, int, int, int, int]:
+    blocks, most = -(-rows // PROMPT_ROWS), max(1, -(-keys // 64))
+    # parts of four tiles at least, about the square root of the keys as above. us by parts: 1 x 30000 keys x 8 kv heads of 128 columns, 48
+    # rows 665 (1), 100 (8), 65 (16), 57 (24), 56 (32); 1 x 4000 85 (1), 25.8 (8), 25.3 (12), 26.5 (16), 36 (32); 1 x 700 21 (1), 16.0
+    # (4), 19.2 (12); 3 x 113 rows x 4 behind 5000 x 8 of 64 82 (1), 39 (4), 35 (5), 40 (6), 37 (8); 1024 x 4 causal rows x 8 of 64 22.9
+    # (1), 20.6 (2), 22.8 (3), of 128 31.3, 29.3, 31.3
+    parts = max(1, min(SLOTS // (units * blocks), most // 4, math.isqrt(keys // 32), 32))
+    return (0, parts, -(-most // parts), units * blocks * parts * PROMPT_ROWS * (D + 4), units * blocks) if parts > 1 else (0, 1, most, 0, 0)
 
 
 def attention8(q: torch.Tensor, cache: Cache8, cu_q: torch.Tensor, ctx_lens: torch.Tensor, block_tables: torch.Tensor, *, n_heads: int,
@@ -247,13 +264,13 @@ def attention8(q: torch.Tensor, cache: Cache8, cu_q: torch.Tensor, ctx_lens: tor
         return out
     keys = max_blocks * cache.block_size if max_k is None else min(max_k, max_blocks * cache.block_size)
     max_q = min(max_q, T)
-    parts, each, floats, tiles = attn8_plan(max_q, H // G, B * G, max(keys, 1), D)
+    form, parts, each, floats, tiles = attn8_plan(max_q, H // G, B * G, max(keys, 1), D)
     st = _stream(dev)
     with _there(dev):
         ws, tickets = _sk_workspace(q.device, st, floats, tiles) if parts > 1 else (None, None)
         check(kernels().loqa_attention8(
             q, ldq, cache.k, cache.v, cache.k_scale, cache.v_scale, cu_q, ctx_lens, block_tables, out, ldo, T, B, H, G, D, cache.block_size,
-            cache.n_blocks, max_blocks, max_q, scale, int(causal), cache.kind, parts, each, ws, 0 if ws is None else ws.numel(), tickets,
+            cache.n_blocks, max_blocks, max_q, scale, int(causal), cache.kind, form, parts, each, ws, 0 if ws is None else ws.numel(), tickets,
             0 if tickets is None else tickets.numel(), st), "attention8")
     return out
 
