@@ -771,13 +771,16 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     constexpr int PER = 256 * (NDT * 16 + 2) * 4;
     const auto rs = __builtin_amdgcn_make_buffer_rsrc(A.ws + unit * A.parts * (PER / 4), 0, A.parts * PER, 0x00020000);
     const int at = part * PER + tid * 16, ml = 256 * NDT * 16 * 4 + tid * 8;
+    const bool some = wave * 32 < rows;                      // a wave without rows leaves nothing
+    if (some) {
 #pragma unroll
-    for (int u = 0; u < 4 * NDT; ++u) {
-      const float4v o = {acc[u / 4][u % 4 * 4], acc[u / 4][u % 4 * 4 + 1], acc[u / 4][u % 4 * 4 + 2], acc[u / 4][u % 4 * 4 + 3]};
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(a8_u4, o), rs, at + u * 4096, 0, 16);
+      for (int u = 0; u < 4 * NDT; ++u) {
+        const float4v o = {acc[u / 4][u % 4 * 4], acc[u / 4][u % 4 * 4 + 1], acc[u / 4][u % 4 * 4 + 2], acc[u / 4][u % 4 * 4 + 3]};
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(a8_u4, o), rs, at + u * 4096, 0, 16);
+      }
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(a8_u2, make_float2(m, l)), rs, part * PER + ml, 0, 16);
     }
-    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(a8_u2, make_float2(m, l)), rs, part * PER + ml, 0, 16);
-    if (!a8_last(A.tickets + unit * TICKET, nparts, reinterpret_cast<int*>(lds))) return;
+    if (!a8_last(A.tickets + unit * TICKET, nparts, reinterpret_cast<int*>(lds)) || !some) return;
     float top = A8_NONE, all = 0.f;
     float tops[A8P_PARTS];                                   // all asked for together
 #pragma unroll
@@ -827,8 +830,9 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   }
 }
 
-// form: 0 prompts, 1 or 2 token steps of up to 16 times as many rows; parts: of a sequence's keys at most; each: tiles of 64 keys of a prompt's part (the longer blocks have more parts); of a token step 1
-// where a wave is expected to have one tile (parts * 128 keys bound the contexts), else 2
+// form: 0 prompts, 1 or 2 token steps of up to 16 times as many rows; parts: of a sequence's keys at most; each: tiles of 64 keys of a
+// prompt's part (the longer blocks have more parts); of a token step 1 where a wave is expected to have one tile (parts * 128 keys bound
+// the contexts), else 2
 extern "C" int loqa_attention8(const void* q, long ldq, const void* k, const void* v, const void* ks, const void* vs, const void* cu,
                                const void* ctx, const void* bt, void* out, long ldo, int T, int B, int H, int G, int D, int blk, int n_blocks,
                                int max_blocks, int max_q, float scale, int causal, int kind, int form, int parts, int each, void* ws, long ws_floats, void* tickets,

@@ -376,6 +376,48 @@ def test_attention_in_parts(dtype, feeds, pasts):
         assert ((got[0].cpu().to(F64) - o).abs() <= oracle.attention_bound(o, mag)).all()
 
 
+@KINDS
+@pytest.mark.parametrize("feeds,pasts,H,G,D,page", [((3, 1, 2), (5, 900, 0), 8, 1, 128, 16), ((5, 5), (1300, 31), 8, 2, 64, 16), ((20, 0, 7), (0, 3, 2000), 4, 4, 64, 32), ((32,), (3000,), 2, 2, 128, 16),
+                                                    ((6, 4, 1), (40, 4100, 2500), 5, 1, 128, 64), ((17, 3), (1, 40000), 1, 1, 64, 16), ((11,), (9000,), 8, 2, 128, 16)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dev", DEVICES)
+def test_attention_of_some_tokens(feeds, pasts, H, G, D, page, dtype, causal, dev):
+    """17 to 48 rows a kv head, contexts that end inside tiles and pages beside ones in many parts, any bound on the keys."""
+    q, cpu, cu, ctx, bt = _attend_case(feeds, pasts, H, G, D, page, dtype, pad=3, spare=8)
+    there = [q.to(dev), _to(cpu, dev), cu.to(dev), ctx.to(dev), bt.to(dev)]
+    o, mag = oracle.attention(q, cpu, cu, ctx, bt, H, causal=causal)
+    rows = int(cu[-1])
+    for max_k in (None, 40, 1000):
+        out = torch.full((q.shape[0], H * D), 3.0, dtype=BF16, device=dev)
+        lowbit.attention8(*there, n_heads=H, max_q=max(feeds), max_k=max_k, causal=causal, out=out)
+        assert (out[rows:] == 3).all()
+        assert ((out.cpu().to(F64) - o).abs()[:rows] <= oracle.attention_bound(o, mag)[:rows]).all()
+
+
+@KINDS
+@pytest.mark.parametrize("dev", DEVICES)
+def test_some_tokens_of_pages_that_are_none(dtype, dev):
+    """24 rows a kv head: contexts of zero, shorter than the feed, on pages that do not exist, codes that are NaN behind the ends."""
+    H, G, D, P, n = 8, 2, 64, 16, 6
+    feeds, ctx = [n] * 5, [0, 1, n // 2, 90, 70]
+    pool, bt = _tables([max(c, 1) for c in ctx], P)
+    cpu = _filled(pool, G, P, D, dtype)
+    free = sorted(set(range(pool)) - {int(bt[b, j]) for b, c in enumerate(ctx) for j in range(-(-max(c, 1) // P))})
+    if dtype is E4M3:
+        cpu.k.view(torch.uint8)[free], cpu.v.view(torch.uint8)[free] = 0x7f, 0x7f
+        used = bt[4, (ctx[4] - 1) // P]
+        cpu.v.view(torch.uint8)[used, :, (ctx[4] - 1) % P + 1:] = 0xff
+        cpu.k.view(torch.uint8)[used, :, (ctx[4] - 1) % P + 1:] = 0xff
+    cpu.k_scale[free], cpu.v_scale[free] = math.nan, math.inf
+    bt[3, 0], bt[3, 1] = pool, -7
+    for b, c in enumerate(ctx):
+        bt[b, -(-max(c, 1) // P):] = free[b % len(free)]
+    q = torch.randn(sum(feeds), H * D, generator=torch.Generator().manual_seed(3)).to(BF16)
+    got = lowbit.attention8(q.to(dev), _to(cpu, dev), _cu(feeds, dev), _i(ctx, dev), bt.to(dev), n_heads=H, max_q=n)
+    assert (got[:2 * n - 1] == 0).all() and got.isfinite().all()
+    _check(got, q, cpu, _cu(feeds), _i(ctx), bt, H)
+
+
 # ------------------------------------------------------------------ pages
 def _pages_case(new, ctx, P, width, free, head=0, spare=2, seed=0):
     held = [-(-c // P) for c in ctx]
