@@ -10,7 +10,6 @@
 // types here with those it knows.
 #include <Python.h>
 #include <ATen/ops/empty.h>
-#include <ATen/ops/narrow.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -249,6 +248,14 @@ at::Tensor made(at::IntArrayRef size, at::ScalarType type, const at::Device& dev
   return at::empty(size, at::TensorOptions().dtype(type).device(dev));
 }
 
+// entries at .. at + m of a vector, as a tensor on the same storage (narrow, without its dispatch: seven of them were half of page_step's call)
+at::Tensor stretch(const at::Tensor& all, long at, long m) {
+  at::Tensor x = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(all.storage()), all.key_set(), all.dtype());
+  x.unsafeGetTensorImpl()->set_storage_offset(all.storage_offset() + at);
+  x.unsafeGetTensorImpl()->set_sizes_contiguous({m});
+  return x;
+}
+
 // (rows x, rows y or None, cu_q, ctx_lens, block_tables, the cache's k; columns of x, of y) -> (T, B, columns of the
 // table, row strides of x and y, y, device)
 PyObject* cache8_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -337,7 +344,7 @@ PyObject* page_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor all = made({B + 1 + 2 * most + B + 2 + 1}, at::kInt, dev), last = made({B}, at::kLong, dev);
     long at = 0;
     auto ints = [&](long m) {
-      const at::Tensor x = all.narrow(0, at, m);
+      const at::Tensor x = stretch(all, at, m);
       at += m;
       return x;
     };
