@@ -144,7 +144,7 @@ def rope_append8(qkv: torch.Tensor, cos_sin: torch.Tensor | None, cache: Cache8,
     qkv: [T, >= (H + 2 Hkv) * D] bf16, q | k | v; cos_sin: [max_pos, D/2, 2] f32 or None (no rotation), which covers every
     position (rows past its end are turned by its last entry). ``max_q`` bounds the rows of a sequence. Rotated keys
     go to their codes without a rounding in between (qkv whose rows do not start at 8 bytes is copied first). Rows at positions below zero or past the block table are not
-    appended. An infinite or NaN entry makes its page's scale so, and with it what attention gives for the page."""
+    appended. No two sequences of a call append to the same page (a shared one ends before the first row that is not shared). An infinite or NaN entry makes its page's scale so, and with it what attention gives for the page."""
     if cache.cuda:
         dev = torch._C._cuda_getDevice()
         q = kernels().rope_append8(qkv, q_out, cu_q, ctx_lens, block_tables, cos_sin, cache.k, cache.v, cache.k_scale, cache.v_scale, n_heads,
@@ -422,7 +422,8 @@ def linear4_plan(M: int, N: int, K: int) -> tuple[int, int, int, int]:
 
 def linear4(x: torch.Tensor, w: Weight4, b: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] bf16 times the transpose of a 4-bit weight (+ bias [N] bf16): [..., N] bf16, summed up in f32. Made for
-    the few rows of token steps; more than 64 read the weight again for every 64. An infinite or NaN entry of x makes its row NaN."""
+    the few rows of token steps; more than 64 read the weight again for every 64. An infinite or NaN entry of x makes its row NaN, and so may
+    one past 2^112 (sums of 143 times a group's entries stay within f32 up to there)."""
     fast = None
     if w.cuda:
         dev = torch._C._cuda_getDevice()
