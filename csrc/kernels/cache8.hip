@@ -11,8 +11,8 @@
 // formulas bit for bit). Where s grows, the page's older rows are rounded again to it.
 // A wave has one page of one head, keys or values, and with it all that touches that scale: no atomics, and the
 // same codes whatever else is in the batch. Bound by latency for token steps (metadata, page number, scale and rows
-// one behind the other: eight replies x 32 + 2 x 8 heads of 128 4.4 us), by the bytes of qkv and q for prompts (2048 such rows, 46 MB, 13.3 us,
-// 3.5 TB/s). Rows of a page are read once and kept where a wave has no more than AP_DEEP of them a lane (331 rows x 5, pages of 32 x 64
+// one behind the other: eight replies x 32 + 2 x 8 heads of 128 4.4 us), by the bytes of qkv and q for prompts (2048 such rows, 46 MB, 13.0 us,
+// 3.6 TB/s; with each head's load behind the store of the one before, and keys and values last, 14.4; 16 bytes a load: no faster). Rows of a page are read once and kept where a wave has no more than AP_DEEP of them a lane (331 rows x 5, pages of 32 x 64
 // columns 8.0 -> 6.4 us).
 struct AppendArgs {
   const bf16_t* qkv;
@@ -24,7 +24,7 @@ struct AppendArgs {
   const int *cu, *ctx, *bt;
   bf16_t* q;
   long long ldq;
-  int T, H, G, sh, n_blocks, max_blocks, max_q, q_wgs;
+  int T, H, G, sh, n_blocks, max_blocks, max_q, kv_wgs;
 };
 
 #define AP_HEADS 4                                // query heads of a thread
@@ -65,18 +65,21 @@ __global__ __launch_bounds__(256) void rope_append8_kernel(AppendArgs A) {
   const int b = blockIdx.y;
   const int q0 = min(max(A.cu[b], 0), A.T), fed = min(max(A.cu[b + 1], q0), A.T) - q0;
   const int n = min(fed, A.max_q), start = A.ctx[b] - fed, end = start + n;
-  if ((int)blockIdx.x < A.q_wgs) {
-    const int chunks = (A.H + AP_HEADS - 1) / AP_HEADS, id = blockIdx.x * 256 + threadIdx.x;
+  if ((int)blockIdx.x >= A.kv_wgs) {              // keys and values, whose chain of loads is the longer, come first
+    const int chunks = (A.H + AP_HEADS - 1) / AP_HEADS, id = (blockIdx.x - A.kv_wgs) * 256 + threadIdx.x;
     const int c = id % LPR * 4, unit = id / LPR, i = unit / chunks, h0 = unit % chunks * AP_HEADS;
     if (i >= n) return;
     ApTurn t;
     if (A.cs) t = ap_turn<D>(A, start + i, c);
     const bf16_t* row = A.qkv + (size_t)(q0 + i) * A.ld;
     bf16_t* out = A.q + (size_t)(q0 + i) * A.ldq;
+    ApPair<D> pairs[AP_HEADS];                    // all asked for ahead of the first store, which q_out may lie in their place
+#pragma unroll
+    for (int u = 0; u < AP_HEADS; ++u) pairs[u] = ap_load<D>(row + min(h0 + u, A.H - 1) * D, c);
 #pragma unroll
     for (int u = 0; u < AP_HEADS; ++u) {
       if (h0 + u >= A.H) break;
-      ApPair<D> p = ap_load<D>(row + (h0 + u) * D, c);
+      ApPair<D>& p = pairs[u];
       if (A.cs) ap_rotate<D>(p, t);
       *reinterpret_cast<uint2*>(out + (h0 + u) * D + c) = make_uint2(pack_bf16x2(p.a[0], p.a[1]), pack_bf16x2(p.a[2], p.a[3]));
       *reinterpret_cast<uint2*>(out + (h0 + u) * D + D / 2 + c) = make_uint2(pack_bf16x2(p.b[0], p.b[1]), pack_bf16x2(p.b[2], p.b[3]));
@@ -84,7 +87,7 @@ __global__ __launch_bounds__(256) void rope_append8_kernel(AppendArgs A) {
     return;
   }
   const int lane = threadIdx.x & 63;
-  const int w = (blockIdx.x - A.q_wgs) * 4 + (threadIdx.x >> 6);
+  const int w = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int values = w & 1, g = (w >> 1) % A.G, pj = (max(start, 0) >> A.sh) + (w >> 1) / A.G;
   const int lo = max(start, pj << A.sh);
   if (n <= 0 || pj >= A.max_blocks || lo >= end) return;
@@ -160,7 +163,7 @@ extern "C" int loqa_rope_append8(const void* qkv, long ld, const void* cs, int c
   const long long pages = ((long long)max_q + blk - 2) / blk + 1, waves = pages * G * 2;   // a feed touches that many pages at most
   const long long wgs = (units + 255) / 256 + (waves + 3) / 4;
   if (units > 1LL << 30 || wgs > 1LL << 24) return (int)hipErrorInvalidValue;
-  a.q_wgs = (int)((units + 255) / 256);
+  a.kv_wgs = (int)((waves + 3) / 4);
   const dim3 grid((unsigned)wgs, B);
 #define GO(D_, K_) hipLaunchKernelGGL((rope_append8_kernel<D_, K_>), grid, dim3(256), 0, st, a)
   if (D == 64) { if (kind == C8_INT8) GO(64, C8_INT8); else GO(64, C8_E4M3); }

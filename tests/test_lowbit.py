@@ -543,6 +543,39 @@ def test_linear4_more_rows(M, N, K, group, zeros, dev):
     assert torch.equal(odd[rows], got[rows]) and not odd[~rows].isfinite().any()
 
 
+@pytest.mark.parametrize("M", [1, 20, 40])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dev", DEVICES)
+def test_linear4_large_entries(M, zeros, dev):
+    """Entries up to 2^112, whose sums with the codes' offset stay finite."""
+    g, N, K, group = torch.Generator().manual_seed(M), 48, 2304, 128
+    codes = torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, generator=g)
+    scales = (2.0 ** -20 * (1 + torch.rand(N, K // group, generator=g))).to(BF16)
+    z = torch.randint(0, 16, (N, K // group), dtype=torch.uint8, generator=g) if zeros else None
+    x = torch.full((M, K), 2.0 ** 112, dtype=BF16)
+    x[:, ::3] *= -0.5
+    w = ref.dense4(codes, scales, z).to(F64)
+    y = x.to(F64) @ w.t()
+    got = lowbit.linear4(x.to(dev), lowbit.Weight4(codes.to(dev), scales.to(dev), z.to(dev) if zeros else None))
+    assert ((got.cpu().to(F64) - y).abs() <= oracle.linear4_bound(y, x, w, scales)).all()
+
+
+@pytest.mark.gpu
+@KINDS
+def test_append_in_place(dtype):
+    """Rotated queries may go where the queries were."""
+    H, G, D, P, n = 6, 2, 64, 16, 50
+    rows = torch.randn(n, (H + 2 * G) * D, generator=torch.Generator().manual_seed(1)).to(BF16).cuda()
+    cs, bt = ref.rope_cos_sin(D, 64, 10000.0).cuda(), torch.arange(4, dtype=I32, device="cuda")[None]
+    a, b = (lowbit.Cache8.empty(4, G, P, D, dtype, "cuda") for _ in range(2))
+    cu, ctx = _i([0, n], "cuda"), _i([n + 3], "cuda")
+    want = lowbit.rope_append8(rows, cs, a, cu, ctx, bt, n_heads=H, max_q=n)
+    out = rows[:, :H * D]
+    assert lowbit.rope_append8(rows, cs, b, cu, ctx, bt, n_heads=H, max_q=n, q_out=out) is out
+    assert torch.equal(out, want)
+    _same(a, b)
+
+
 @pytest.mark.gpu
 def test_linear4_parts_in_graphs_and_streams():
     """Products in parts of K: a captured one replayed between eager ones, and two streams at once."""
