@@ -641,10 +641,10 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     ask(kt + A8P_KEYS);
     asked(kt + A8P_KEYS);
   }
-  // A tile: the scores of its first 32 keys, beside which the next tile is widened; those of the second 32 beside the weights of the
-  // first, to the reference as it stands; the maxima, which move it where they have to (then the weights are taken once more); the
-  // values' products of the first 32 keys beside the weights of the second; those of the second beside the addresses of the tile after
-  // the next. (One after the other, stages toggled in registers: the 2048 rows above 58 us, 56 now.)
+  // A tile: the scores of its first 32 keys, beside which the next tile is widened; those of the second 32; the maxima, which move the
+  // reference where they have to, and the weights of the first keys; the values' products of these beside the weights of the second;
+  // those of the second beside the addresses of the tile after the next. (One after the other, stages toggled in registers: the 2048
+  // rows above 58 us, 56 now; the first weights beside the second scores, and once more where the reference moves: no faster.)
   constexpr int KR = 4, VR = 4;                              // fragments in flight + 1
   // rows of this wave that some key of a tile from here on is hidden from, or that end in it
   const int edge = min(f.keys, A.causal ? f.past + (r0 + wave * 32) / Gq + 1 : f.keys) - A8P_KEYS;
@@ -707,22 +707,21 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
       const float k = factor * ks[g];
       c[g] = k < 1.1754943508222875e-38f ? 1.1754943508222875e-38f : k;     // of no use to a masked -infinity if zero; NaN stays
     }
-    if (kt > edge) hide(0);
-    constexpr int SW = 16 / NS;                              // scores a step
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
       s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[(NS + u) % KR], qf[u], u == 0 ? zero : s[1], 0, 0, 0);
       if (u + KR - 1 < NS) kread(NS + u + KR - 1);
-      weights(u * SW / 8, u * SW % 8, u * SW % 8 + SW);
-      tops(u * SW / 8, u * SW % 8, u * SW % 8 + SW);
       __builtin_amdgcn_sched_barrier(0);
     }
     store_scales(1 - stage);
 #pragma unroll
     for (int v = 0; v < VR - 1; ++v) vread(v);
-    if (kt > edge) hide(1);
-    tops(2, 0, 8);
-    tops(3, 0, 8);
+    if (kt > edge) {
+      hide(0);
+      hide(1);
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) tops(g, 0, 8);
     // x c + log2 vs with c above zero: the largest product of a group is its largest score
     float mx = -INFINITY;
 #pragma unroll
@@ -738,9 +737,9 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
       for (int d = 0; d < NDT; ++d)
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[d][j] *= alpha;
-      weights(0, 0, 8);
-      weights(1, 0, 8);
     }
+    weights(0, 0, 8);
+    weights(1, 0, 8);
     __builtin_amdgcn_sched_barrier(0);
     constexpr int PW = 16 / (2 * NDT);
 #pragma unroll
