@@ -501,7 +501,7 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R, RT>::FIT)) void attn8
 // the longest parts first, counted by a lane for each block (2048 rows 79); six and eight fragments of K in flight, halves of a chunk
 // swapped against bank conflicts of the writes (nothing); a wave's priority raised for products or for weights, the maxima in 16
 // instructions fewer, the first weights pinned beside the second scores (nothing, 1 % at most); a long and a short block one behind the
-// other in a workgroup (57).
+// other in a workgroup (57); 64 rows a wave, half the reads of LDS (64 columns: no faster; 128 do not fit the registers).
 #define A8P_ROWS 128
 #define A8P_KEYS 64
 #define A8P_PARTS 32
