@@ -387,12 +387,15 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R, RT>::FIT)) void attn8
 #pragma unroll
         for (int j = 0; j < 4; ++j) st[r][t][j] = fmaf(st[r][t][j], c, lv[t]);
       }
+      float per[2] = {inv[0], inv[1]};           // of a page that the row sees no key of (it may be another sequence's, its scale no number): 0
       if (edge) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+          if (kt + 16 * t > seen[r]) per[t] = 0.f;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (kt + 16 * t + 4 * fq + j > seen[r]) st[r][t][j] = -INFINITY;
+        }
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -416,7 +419,7 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R, RT>::FIT)) void attn8
           sum += e;
           p[r][4 * t + j] = (_Float16)e;
         }
-        l_run[r] = fmaf(sum, inv[t], l_run[r]);  // of this lane's keys
+        l_run[r] = fmaf(sum, per[t], l_run[r]);  // of this lane's keys
       }
     }
 #pragma unroll

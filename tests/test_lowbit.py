@@ -418,6 +418,28 @@ def test_some_tokens_of_pages_that_are_none(dtype, dev):
     _check(got, q, cpu, _cu(feeds), _i(ctx), bt, H)
 
 
+@KINDS
+@pytest.mark.parametrize("n,H,G,D", [(1, 8, 2, 128), (3, 4, 1, 64), (6, 4, 1, 128), (20, 4, 2, 64)])
+@pytest.mark.parametrize("dev", DEVICES)
+def test_pages_behind_a_context_are_no_part_of_it(dtype, n, H, G, D, dev):
+    """Contexts that end in either half of a tile, with table entries behind them that name pages whose scales are NaN: the
+    padding of a table, or what an ended sequence left."""
+    P = 16
+    ctx = [20, 33, 48, 64, 300, 321, 37]
+    feeds = [n] * len(ctx)
+    pool, bt = _tables(ctx, P, width=24)
+    cpu = _filled(pool, G, P, D, dtype)
+    used = {int(bt[b, j]) for b, c in enumerate(ctx) for j in range(-(-c // P))}
+    free = sorted(set(range(pool)) - used)
+    cpu.k_scale[free], cpu.v_scale[free] = math.nan, math.nan
+    for b, c in enumerate(ctx):
+        bt[b, -(-c // P):] = free[b % len(free)]
+    q = torch.randn(sum(feeds), H * D, generator=torch.Generator().manual_seed(3)).to(BF16)
+    got = lowbit.attention8(q.to(dev), _to(cpu, dev), _cu(feeds, dev), _i(ctx, dev), bt.to(dev), n_heads=H, max_q=n)
+    assert got.isfinite().all()
+    _check(got, q, cpu, _cu(feeds), _i(ctx), bt, H)
+
+
 # ------------------------------------------------------------------ pages
 def _pages_case(new, ctx, P, width, free, head=0, spare=2, seed=0):
     held = [-(-c // P) for c in ctx]
