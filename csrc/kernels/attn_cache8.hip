@@ -656,7 +656,8 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     const int kt = (i0 + i) * A8P_KEYS;
     fl_meet();                                               // this stage is written, nobody reads the other one any more; loads stay under way
     const float* sc = reinterpret_cast<const float*>(lds + L::SCALES + stage * 64);
-    const float4v ks = *reinterpret_cast<const float4v*>(sc), lv = *reinterpret_cast<const float4v*>(sc + 4), inv = *reinterpret_cast<const float4v*>(sc + 8);
+    const float4v ks = *reinterpret_cast<const float4v*>(sc);
+    float4v lv = *reinterpret_cast<const float4v*>(sc + 4), inv = *reinterpret_cast<const float4v*>(sc + 8);
     float16v s[2];
     c8_h8 kf[KR], vf[VR], p[4];
     float sum[4], c[4], top[4];
@@ -722,6 +723,13 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     if (kt > edge) {
       hide(0);
       hide(1);
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (kt + 16 * g > seen) {                            // keys that the row sees none of: their page's scales, which may be no numbers, are not its own
+          c[g] = 1.f;
+          lv[g] = -INFINITY;
+          inv[g] = 0.f;
+        }
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) tops(g, 0, 8);

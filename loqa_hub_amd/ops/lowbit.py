@@ -144,7 +144,8 @@ def rope_append8(qkv: torch.Tensor, cos_sin: torch.Tensor | None, cache: Cache8,
     qkv: [T, >= (H + 2 Hkv) * D] bf16, q | k | v; cos_sin: [max_pos, D/2, 2] f32 or None (no rotation), which covers every
     position (rows past its end are turned by its last entry). ``max_q`` bounds the rows of a sequence. Rotated keys
     go to their codes without a rounding in between (qkv whose rows do not start at 8 bytes is copied first). Rows at positions below zero or past the block table are not
-    appended. No two sequences of a call append to the same page (a shared one ends before the first row that is not shared). An infinite or NaN entry makes its page's scale so, and with it what attention gives for the page."""
+    appended. No two sequences of a call append to the same page (a shared one ends before the first row that is not shared). An infinite or NaN entry makes its page's scale so, and with it
+    what attention gives to rows that see a key of the page; rows ahead of the page and other sequences are as without it."""
     if cache.cuda:
         dev = torch._C._cuda_getDevice()
         q = kernels().rope_append8(qkv, q_out, cu_q, ctx_lens, block_tables, cos_sin, cache.k, cache.v, cache.k_scale, cache.v_scale, n_heads,

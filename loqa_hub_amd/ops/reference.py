@@ -1526,7 +1526,12 @@ def attention8(q, cache, cu_q, ctx_lens, block_tables, *, n_heads, max_q, causal
         e = torch.exp(w - torch.where(top == -math.inf, torch.zeros_like(top), top))
         total = e.sum(-1, keepdim=True)
         p = e / torch.where(total == 0, torch.ones_like(total), total)
-        out[q0:q0 + n, :H * D] = torch.einsum("hij,jhd->ihd", p, v.repeat_interleave(H // G, 1)).reshape(n, H * D).to(out.dtype)
+        v = v.repeat_interleave(H // G, 1)
+        if v.isfinite().all():
+            o = torch.einsum("hij,jhd->ihd", p, v)
+        else:                                          # 0 * NaN: of each row, the keys that it sees
+            o = torch.stack([torch.einsum("hj,jhd->hd", p[:, i, ~hide[i]], v[~hide[i]]) for i in range(n)])
+        out[q0:q0 + n, :H * D] = o.reshape(n, H * D).to(out.dtype)
     return out
 
 

@@ -440,6 +440,26 @@ def test_pages_behind_a_context_are_no_part_of_it(dtype, n, H, G, D, dev):
     _check(got, q, cpu, _cu(feeds), _i(ctx), bt, H)
 
 
+@KINDS
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("x", [math.nan, math.inf])
+@pytest.mark.parametrize("n,past,H,D,P", [(12, 40, 1, 64, 16), (12, 25, 2, 128, 32), (40, 10, 1, 64, 16), (70, 100, 2, 128, 64), (150, 0, 4, 64, 16)])
+@pytest.mark.parametrize("dev", DEVICES)
+def test_rows_ahead_of_a_page_that_is_no_number(n, past, H, D, P, x, which, dtype, dev):
+    """A page whose scale is no number is that to rows that see one of its keys, and nothing to those ahead of it."""
+    q, cpu, cu, ctx, bt = _attend_case((n,), (past,), H, 1, D, P, dtype)
+    page = (past + n // 2) // P + 1 if (past + n // 2) // P + 1 < bt.shape[1] else (past + n // 2) // P
+    ahead = max(page * P - past, 0)                      # rows that see none of it
+    assert 0 < ahead < n
+    spoilt = _to(cpu, dev)
+    getattr(spoilt, which)[int(bt[0, page])] = x
+    got = lowbit.attention8(q.to(dev), spoilt, cu.to(dev), ctx.to(dev), bt.to(dev), n_heads=H, max_q=n).cpu()
+    o, mag = oracle.attention(q, cpu, cu, ctx, bt, H)
+    assert ((got.to(F64) - o).abs()[:ahead] <= oracle.attention_bound(o, mag)[:ahead]).all()
+    if math.isnan(x):
+        assert got[ahead:].isnan().all()
+
+
 # ------------------------------------------------------------------ pages
 def _pages_case(new, ctx, P, width, free, head=0, spare=2, seed=0):
     held = [-(-c // P) for c in ctx]
