@@ -4,17 +4,22 @@
 //   x_j = q . k_j (f16 MFMAs, f32 sums),  s_j = scale log2(e) ks x_j,  o = sum_j 2^(s_j) vs v_j / sum_j 2^(s_j)
 //
 // with ks, vs of a key's page. The values' scale goes into the exponent: t_j = s_j + log2(vs), weights w_j = 2^(t_j - m)
-// are what the codes of v are summed up with, and the denominator is sum_j w_j / vs in f32. The reference m of a row follows its
-// largest t_j within a factor of 2^8, so weights are f16 without a range of their own: 11 bits each, under 2^-14 an absolute 2^-25
-// (with a reference that never lags, some row of a wave has a new maximum in nearly every tile, and rescaling is a tenth
-// of a tile's instructions). Queries enter as f16 times a power of two of
+// are what the codes of v are summed up with, and the denominator is sum_j w_j / vs in f32. The reference m of a row starts 2^7 below its
+// largest t_j and follows it within a factor of 2^8, so weights reach 2^15 and are f16 without a range of their own: 11 bits each, under
+// 2^-14 an absolute 2^-25. The largest is 2^7 or more, so what becomes zero there is under 2^-32 of it, and n such keys, which the f32
+// denominator still counts, lose 2^-32 n (with a reference at the largest, 2^-25 n: 3 % of a million). With a reference that never lags, some
+// row of a wave has a new maximum in nearly every tile, and rescaling is a tenth of a tile's instructions. The denominator is
+// summed up 2^7 smaller, for the room that scales of 2^-100 leave it. Queries enter as f16 times a power of two of
 // the row that puts its largest entry in 2^14 .. 2^15: bf16's 8 bits are exact down to 2^-28 of it.
 //
 // Rows that see no key (a position before the first) give zeros; keys of pages that do not exist count as masked.
 #include "cache8.h"
 #include "flash_pipe.h"
 
-#define A8_NONE -3.0e38f                           // a row's maximum before its first key
+#define A8_NONE -3.0e38f                           // a row's reference before its first key
+#define A8_BELOW 7.f                               // of a largest score, the reference that it sets
+#define A8_MOST 15.f                               // of a weight, as a power of two: then the reference moves
+#define A8_DOWN 0.0078125f                         // 2^-7, of the denominator
 
 struct Attn8Args {
   const bf16_t* q;
@@ -114,7 +119,7 @@ __device__ __forceinline__ bool a8_last(int* ticket, int n, int* flag) {
 
 __device__ __forceinline__ void a8_put(bf16_t* at, const float4v& o, float l, bool whole) {
   const float inv = l == 0.f ? 0.f : 1.f / l;     // NaN stays
-  const uint2 w = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+  const uint2 w = make_uint2(pack_bf16x2(o[0] * A8_DOWN * inv, o[1] * A8_DOWN * inv), pack_bf16x2(o[2] * A8_DOWN * inv, o[3] * A8_DOWN * inv));
   if (whole) {
     *reinterpret_cast<uint2*>(at) = w;
   } else {
@@ -375,7 +380,7 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R, RT>::FIT)) void attn8
       const float vs = a8_least(sc[2 + t]);
       ks[t] = there ? a8_least(sc[t]) : 0.f;
       lv[t] = there ? __builtin_amdgcn_logf(vs) : -INFINITY;
-      inv[t] = there ? __builtin_amdgcn_rcpf(vs) : 0.f;
+      inv[t] = there ? __builtin_amdgcn_rcpf(vs) * A8_DOWN : 0.f;
     }
     const bool edge = kt + A8_TILE > kend || (A.causal && kt + A8_TILE - 1 > f.past);
     c8_h8 p[RT];
@@ -401,8 +406,8 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R, RT>::FIT)) void attn8
 #pragma unroll
       for (int j = 0; j < 8; ++j) mx = fmaxf(mx, st[r][j >> 2][j & 3]);
       mx = a8_max16(fl_max32(mx));
-      if (__any(mx > m_run[r] + 8.f)) {          // as in the prompt form
-        const float m_new = fmaxf(m_run[r], mx), alpha = __builtin_amdgcn_exp2f(m_run[r] - m_new);
+      if (__any(mx > m_run[r] + A8_MOST)) {      // as in the prompt form
+        const float m_new = fmaxf(m_run[r], mx - A8_BELOW), alpha = __builtin_amdgcn_exp2f(m_run[r] - m_new);
         m_run[r] = m_new;
         l_run[r] *= alpha;
 #pragma unroll
@@ -604,7 +609,7 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
       const float vs = a8_least(sv);
       s[0] = there ? a8_least(sk) : 1.f;
       s[4] = there ? __builtin_amdgcn_logf(vs) : -INFINITY;
-      s[8] = there ? __builtin_amdgcn_rcpf(vs) : 0.f;        // off by 2^-23
+      s[8] = there ? __builtin_amdgcn_rcpf(vs) * A8_DOWN : 0.f;        // off by 2^-23
     }
   };
 
@@ -737,11 +742,11 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     float mx = -INFINITY;
 #pragma unroll
     for (int g = 0; g < 4; ++g) mx = fmaxf(mx, fmaf(top[g], c[g], lv[g]));
-    // the reference stays where it is while no row's maximum passes it by more than a factor of 2^8: f16 weights keep their 11
-    // bits up to 2^15, and a prompt's first tiles nearly always raise some row of the wave
+    // the reference stays where it is while no weight passes 2^15, up to which f16 keeps 11 bits: a prompt's first tiles nearly
+    // always raise some row of the wave
     mx = fl_max32(mx);
-    if (__any(mx > m + 8.f)) {
-      const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
+    if (__any(mx > m + A8_MOST)) {
+      const float m_new = fmaxf(m, mx - A8_BELOW), alpha = __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
       l *= alpha;
 #pragma unroll
@@ -832,8 +837,10 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     const float by = l == 0.f ? 0.f : 1.f / l;               // NaN stays
 #pragma unroll
     for (int u = 0; u < 4 * NDT; ++u) {                      // accumulators 4 u ..: columns 8 u + 4 h ..
-      const uint2 w = make_uint2(pack_bf16x2(acc[u / 4][u % 4 * 4] * by, acc[u / 4][u % 4 * 4 + 1] * by),
-                                 pack_bf16x2(acc[u / 4][u % 4 * 4 + 2] * by, acc[u / 4][u % 4 * 4 + 3] * by));
+      float o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = acc[u / 4][u % 4 * 4 + j] * A8_DOWN * by;
+      const uint2 w = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
       if (whole) {
         *reinterpret_cast<uint2*>(at + 8 * u) = w;
       } else {

@@ -460,6 +460,34 @@ def test_rows_ahead_of_a_page_that_is_no_number(n, past, H, D, P, x, which, dtyp
         assert got[ahead:].isnan().all()
 
 
+@KINDS
+@pytest.mark.parametrize("H", [1, 20, 40])
+@pytest.mark.parametrize("dev", DEVICES)
+def test_many_keys_behind_a_dominant_one(dtype, H, dev):
+    """2^18 keys of like weight, 2^-26.5 of the first one's, whose values are zero: what they sum up to is the result. A weight
+    is f16 over a reference 2^7 below the row's largest one: off by 2^-11, or by 2^-25 of 2^7 under 2^-14 of it; in one part, so that
+    all of them follow the first key."""
+    D, P, L, code = 64, 16, 1 << 18, 64
+    pages = L // P
+    cache = lowbit.Cache8.empty(pages, 1, P, D, dtype)
+    cache.k_scale.fill_(1 / code)
+    cache.v_scale.fill_(1 / code)
+    for t in (cache.k, cache.v):
+        t[0, 0, 0] = 0
+    cache.k[0, 0, 0, 0] = code
+    ones = torch.full((D,), code, dtype=torch.float32).to(dtype)
+    cache.v.view(torch.uint8)[:] = ones.view(torch.uint8)
+    cache.v.view(torch.uint8)[0, 0, 0] = 0
+    q = torch.zeros(1, H * D, dtype=BF16)
+    q[0, ::D] = 26.5 * math.log(2)
+    w = math.exp(-float(q[0, 0]))
+    total = (L - 1) * w
+    o = total / (1 + total)
+    bt = torch.arange(pages, dtype=I32, device=dev)[None]
+    got = lowbit.attention8(q.to(dev), _to(cache, dev), _i([0, 1], dev), _i([L], dev), bt, n_heads=H, max_q=1, max_k=1, scale=1.0).cpu().to(F64)
+    assert ((got - o).abs() <= (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -14) * o + L * 2.0 ** -32).all(), (float(got.min()), float(got.max()), o)
+
+
 # ------------------------------------------------------------------ pages
 def _pages_case(new, ctx, P, width, free, head=0, spare=2, seed=0):
     held = [-(-c // P) for c in ctx]
