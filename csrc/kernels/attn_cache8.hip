@@ -48,8 +48,6 @@ __device__ __forceinline__ A8Feed a8_feed(const Attn8Args& A, int b) {
   return f;
 }
 
-__device__ __forceinline__ float a8_least(float s) { return s < C8_LEAST ? C8_LEAST : s; }   // NaN stays
-
 // N pieces of eight entries of a query row, piece u at at(u), asked for together (rows at odd places entry by entry)
 template <int N, typename At> __device__ __forceinline__ void a8_row(const Attn8Args& A, uint4 (&x)[N], At&& at) {
   if ((((size_t)A.q | (size_t)A.ldq * 2) & 15) == 0) {
@@ -377,8 +375,8 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R, RT>::FIT)) void attn8
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const bool there = (unsigned)(t ? pa1 : pa0) < (unsigned)A.n_blocks;
-      const float vs = a8_least(sc[2 + t]);
-      ks[t] = there ? a8_least(sc[t]) : 0.f;
+      const float vs = c8_least(sc[2 + t]);
+      ks[t] = there ? c8_least(sc[t]) : 0.f;
       lv[t] = there ? __builtin_amdgcn_logf(vs) : -INFINITY;
       inv[t] = there ? __builtin_amdgcn_rcpf(vs) * A8_DOWN : 0.f;
     }
@@ -606,8 +604,8 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   auto store_scales = [&](int stage) __attribute__((always_inline)) {
     if (tid < 4) {
       float* s = reinterpret_cast<float*>(lds + L::SCALES + stage * 64) + tid;
-      const float vs = a8_least(sv);
-      s[0] = there ? a8_least(sk) : 1.f;
+      const float vs = c8_least(sv);
+      s[0] = there ? c8_least(sk) : 1.f;
       s[4] = there ? __builtin_amdgcn_logf(vs) : -INFINITY;
       s[8] = there ? __builtin_amdgcn_rcpf(vs) * A8_DOWN : 0.f;        // off by 2^-23
     }

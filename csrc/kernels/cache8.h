@@ -4,7 +4,7 @@
 // Pages [n_blocks, Hkv, BLK, D] of int8 or OCP e4m3 codes; an f32 scale per page and head, of keys and of
 // values: an entry stands for code * scale. Both kinds of codes are f16 values exactly (int8: 1024 + (c + 128)
 // formed by bytes, less 1152; e4m3: the hardware's conversion), so products run on the f16 MFMAs without
-// a rounding of what is cached. A scale under C8_LEAST counts as C8_LEAST.
+// a rounding of what is cached. A scale under C8_LEAST (a negative one too) counts as C8_LEAST to all that read it.
 #pragma once
 #include "common.h"
 
@@ -16,6 +16,8 @@ typedef _Float16 c8_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 c8_h8 __attribute__((ext_vector_type(8)));
 typedef unsigned c8_u2 __attribute__((ext_vector_type(2)));
 typedef unsigned c8_u4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float c8_least(float s) { return s < C8_LEAST ? C8_LEAST : s; }   // NaN stays
 
 // four codes -> four f16
 template <int KIND> __device__ __forceinline__ c8_u2 c8_widen(unsigned w) {

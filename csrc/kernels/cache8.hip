@@ -100,7 +100,8 @@ __global__ __launch_bounds__(256) void rope_append8_kernel(AppendArgs A) {
   const bool turn = A.cs && !values;
   const int c = lane % LPR * 4, r0 = lane / LPR;
   const bf16_t* src = A.qkv + (size_t)(q0 + lo - start) * A.ld + (size_t)(A.H + (values ? A.G : 0) + g) * D;
-  const unsigned had = off > 0 ? __float_as_uint(*scale) & 0x7fffffffu : 0u;
+  const float before = off > 0 ? *scale : 0.f;
+  const unsigned had = off > 0 ? __float_as_uint(c8_least(before)) & 0x7fffffffu : 0u;
   // AP_DEEP rows of a lane under way together; a page of no more than that is read once
   constexpr int DEEP = AP_DEEP * RPW;
   ApPair<D> p[AP_DEEP];
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(256) void rope_append8_kernel(AppendArgs A) {
       *reinterpret_cast<unsigned*>(codes + (off + r) * D + D / 2 + c) = c8_codes<KIND>(p[i].b, s);
     }
   }
-  if (lane == 0 && (off == 0 || now != had)) *scale = s;
+  if (lane == 0 && (off == 0 || now != __float_as_uint(before))) *scale = s;
 }
 
 extern "C" int loqa_rope_append8(const void* qkv, long ld, const void* cs, int cs_rows, void* k, void* v, void* ks, void* vs, const void* cu,
@@ -204,7 +205,7 @@ __global__ __launch_bounds__(256) void read8_kernel(Read8Args A) {
   if ((unsigned)page < (unsigned)A.n_blocks) {
     const size_t at = (size_t)page * A.G + g, off = ((at << A.sh) + (pos & ((1 << A.sh) - 1))) * D + c * 8;
     const uint2 x = *reinterpret_cast<const uint2*>(A.k + off), y = *reinterpret_cast<const uint2*>(A.v + off);
-    const float sk = A.ks[at], sv = A.vs[at];
+    const float sk = c8_least(A.ks[at]), sv = c8_least(A.vs[at]);
     const float4v a = c8_floats<KIND>(x.x), b = c8_floats<KIND>(x.y), e = c8_floats<KIND>(y.x), f = c8_floats<KIND>(y.y);
     ko = make_uint4(pack_bf16x2(a[0] * sk, a[1] * sk), pack_bf16x2(a[2] * sk, a[3] * sk), pack_bf16x2(b[0] * sk, b[1] * sk), pack_bf16x2(b[2] * sk, b[3] * sk));
     vo = make_uint4(pack_bf16x2(e[0] * sv, e[1] * sv), pack_bf16x2(e[2] * sv, e[3] * sv), pack_bf16x2(f[0] * sv, f[1] * sv), pack_bf16x2(f[2] * sv, f[3] * sv));

@@ -75,7 +75,8 @@ class Cache8:
     A page's scale starts anew with the row at its first place and only grows until the next such row; its
     older rows are rounded again where it grows, so a page filled row by row is off by up to a step where one filled at
     once is off by half a step. e4m3 scales are powers of two, whose growth rounds nothing again but the smallest
-    entries. Scales below 2^-100 count as 2^-100. Page sizes are powers of two from 16 on."""
+    entries. Scales below 2^-100, negative ones among them, count as 2^-100 everywhere. Page sizes are
+    powers of two from 16 on."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "kind", "n_blocks", "n_kv", "block_size", "head_dim", "cuda")
 

@@ -1479,7 +1479,7 @@ def rope_append8(qkv, cos_sin, cache, cu_q, ctx_lens, block_tables, *, n_heads, 
             off = lo - p
             for codes, scale, new in ((cache.k, cache.k_scale, qk[:, H:]), (cache.v, cache.v_scale, v)):
                 rows = new[lo - start:hi - start].transpose(0, 1)              # [G, rows, D]
-                had = scale[page].clone()
+                had = scale[page].clamp_min(SCALE_LEAST)
                 now = torch.maximum(page_scale8(rows.abs().amax((1, 2)), dtype), had if off else torch.zeros_like(had))
                 now = torch.where(now < SCALE_LEAST, torch.full_like(now, SCALE_LEAST), now)
                 if off:
@@ -1498,8 +1498,8 @@ def read8(cache, cu_k, first, block_tables, k, v):
             pos = int(first[b]) + i
             page = int(block_tables[b, pos // P]) if 0 <= pos < P * block_tables.shape[1] else -1
             if 0 <= page < cache.n_blocks:
-                k[at + i] = (cache.k[page, :, pos % P].float() * cache.k_scale[page][:, None]).to(k.dtype)
-                v[at + i] = (cache.v[page, :, pos % P].float() * cache.v_scale[page][:, None]).to(v.dtype)
+                k[at + i] = (cache.k[page, :, pos % P].float() * cache.k_scale[page].clamp_min(SCALE_LEAST)[:, None]).to(k.dtype)
+                v[at + i] = (cache.v[page, :, pos % P].float() * cache.v_scale[page].clamp_min(SCALE_LEAST)[:, None]).to(v.dtype)
     return k, v
 
 

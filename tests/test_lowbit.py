@@ -246,6 +246,35 @@ def test_read(dtype, dev, D, P):
         assert all(t.shape == (total, G, D) and (t == 0).all() for t in none)
 
 
+@KINDS
+@pytest.mark.parametrize("had", [0.0, -0.0, 2.0 ** -120, -0.5, 2.0 ** -101])
+@pytest.mark.parametrize("dev", DEVICES)
+def test_scales_below_the_least(dtype, had, dev):
+    """They count as 2^-100 to whatever reads them: rows back, attention, and older rows that are rounded again."""
+    G, D, P, least = 2, 64, 16, 2.0 ** -100
+    base = _filled(3, G, P, D, dtype)
+    base.k_scale[1], base.v_scale[1] = had, had
+    bt = _i([[1]], dev)
+    codes = {n: getattr(base, n)[1].float() for n in ("k", "v")}
+    k, v = lowbit.read8(_to(base, dev), _i([0, 9], dev), _i([0], dev), bt, total=9)
+    for got, n in ((k, "k"), (v, "v")):
+        assert torch.equal(got.cpu(), (codes[n][:, :9].transpose(0, 1) * least).to(BF16))
+    q = torch.randn(1, 2 * D, generator=torch.Generator().manual_seed(1)).to(BF16)
+    _check(lowbit.attention8(q.to(dev), _to(base, dev), _i([0, 1], dev), _i([9], dev), bt, n_heads=2, max_q=1), q, base, _i([0, 1]), _i([9]), bt.cpu(), 2)
+    # a row that asks for less than the least scale changes no older one; one that asks for 2^-99 halves them; a large one leaves zeros
+    top = 127.0 if dtype is INT8 else 448.0
+    for row, now, keep in ((2.0 ** -115, least, lambda c: c), (top * 2.0 ** -99, 2.0 ** -99, lambda c: ref.codes8(c / 2, dtype).float()),
+                           (top, 1.0, lambda c: torch.zeros_like(c))):
+        cache = _to(base, dev)
+        x = torch.zeros(1, 3 * 2 * D, dtype=BF16)
+        x[0, 2 * D:] = row
+        lowbit.rope_append8(x.to(dev), None, cache, _i([0, 1], dev), _i([10], dev), bt, n_heads=2, max_q=1)
+        for n in ("k", "v"):
+            s, c = getattr(cache, n + "_scale")[1].cpu(), getattr(cache, n)[1].cpu().float()
+            assert (s == now).all() and torch.equal(c[:, :9], keep(codes[n][:, :9])) and torch.equal(c[:, 10:], codes[n][:, 10:])
+            assert (c[:, 9] == (0 if row < least else top)).all()
+
+
 # ------------------------------------------------------------------ attention
 def _attend_case(feeds, pasts, H, G, D, page, dtype, seed=0, std=1.5, pad=0, spare=0):
     g = torch.Generator().manual_seed(seed + 1)
