@@ -286,7 +286,7 @@ PyObject* rope_append8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor &x = *t[0], &bt = *t[4];
     const at::Device dev = t[6]->device();
     const long H = v[0], G = v[1], D = v[2];
-    if (!rows_on(x, (H + 2 * G) * D, dev) || (t[1] && (!rows_on(*t[1], H * D, dev) || t[1]->size(0) != x.size(0)))) Py_RETURN_NONE;
+    if (H <= 0 || !rows_on(x, (H + 2 * G) * D, dev) || (t[1] && (!rows_on(*t[1], H * D, dev) || t[1]->size(0) != x.size(0)))) Py_RETURN_NONE;
     if (!i32_on(t[2], dev) || !i32_on(t[3], dev) || !i32_on(t[4], dev)) Py_RETURN_NONE;
     const long T = x.size(0), B = t[3]->numel();
     if (T == 0 || B == 0 || v[5] <= 0 || t[2]->numel() != B + 1 || bt.dim() != 2 || bt.size(0) != B || bt.size(1) == 0) Py_RETURN_NONE;
@@ -338,7 +338,7 @@ PyObject* page_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const long B = t[0]->numel(), pool = t[3]->numel(), P = v[0], most = v[1];
     if (B == 0 || B > v[2] || t[1]->numel() != B || bt.dim() != 2 || bt.size(0) != B || bt.size(1) == 0 || t[4]->numel() != 2 || pool == 0)
       Py_RETURN_NONE;
-    if (most < 0 || most > 1L << 30 || P <= 0 || (P & (P - 1)) || pool * P >= 1L << 31) Py_RETURN_NONE;
+    if (most < 0 || most > 1L << 30 || P <= 0 || (P & (P - 1)) || P >= 1L << 31 || pool * P >= 1L << 31) Py_RETURN_NONE;
     if ((t[5] && t[5]->numel() != B) || (t[6] && t[6]->numel() != 2)) Py_RETURN_NONE;
     // one allocation for all that is int32
     const at::Tensor all = made({B + 1 + 2 * most + B + 2 + 1}, at::kInt, dev), last = made({B}, at::kLong, dev);

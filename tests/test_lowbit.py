@@ -906,3 +906,68 @@ def test_refusals_of_pages_and_products():
     for args in ((torch.zeros(4, 100), 64), (torch.zeros(4, 128), 16), (torch.zeros(128), 64)):
         with pytest.raises(ValueError):
             lowbit.quantize4(*args)
+
+
+def _there(x):
+    """On the GPU, with a stride where it had one."""
+    if not isinstance(x, torch.Tensor):
+        return x
+    return x.cuda() if x.is_contiguous() else x.cuda().repeat_interleave(2, 1)[:, ::2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("change,error", [
+    (dict(cu_q=torch.tensor([0, 2])), TypeError), (dict(ctx_lens=torch.tensor([2.0])), TypeError), (dict(block_tables=_i([0, 1])), ValueError),
+    (dict(block_tables=_i([[0], [1]])), ValueError), (dict(cu_q=_i([0, 1, 2])), ValueError), (dict(block_tables=torch.zeros(1, 0, dtype=I32)), ValueError),
+    (dict(block_tables=_i([[0, 1, 2, 3]])[:, ::2]), ValueError), (dict(n_heads=0), ValueError), (dict(n_heads=-1), ValueError), (dict(max_q=-1), ValueError)])
+def test_refusals_of_sequences_on_the_gpu(change, error):
+    """The same calls are refused, in the same way, where the checks are the launch module's."""
+    a = {**_good("cuda"), **{k: _there(v) for k, v in change.items()}}
+    with pytest.raises(error):
+        lowbit.attention8(torch.zeros(2, 256, dtype=BF16, device="cuda"), **a)
+    with pytest.raises(error):
+        lowbit.rope_append8(torch.zeros(2, 512, dtype=BF16, device="cuda"), None, **a)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    rows, there = lambda *s: torch.zeros(*s, dtype=BF16, device="cuda"), dict(device="cuda")
+    good = _good("cuda")
+    cache = good["cache"]
+    for name in ("cu_q", "ctx_lens", "block_tables"):            # one tensor on the CPU
+        for fn, args in ((lowbit.attention8, (rows(2, 256),)), (lowbit.rope_append8, (rows(2, 512), None))):
+            with pytest.raises(ValueError):
+                fn(*args, **{**good, name: good[name].cpu()})
+    for kw in (dict(q=torch.zeros(2, 256, **there)), dict(q=rows(2, 255)), dict(q=rows(2, 512)[:, ::2]), dict(q=rows(2, 256).cpu()), dict(q=rows(2, 4, 64)),
+               dict(out=rows(1, 256)), dict(out=torch.zeros(2, 256, **there)), dict(out=rows(1, 256).expand(2, 256)), dict(n_heads=3), dict(max_k=-1)):
+        a = {**good, "q": rows(2, 256), **kw}
+        with pytest.raises((TypeError, ValueError)):
+            lowbit.attention8(a.pop("q"), **a)
+    for kw in (dict(qkv=rows(2, 511)), dict(qkv=torch.zeros(2, 512, **there)), dict(qkv=rows(2, 512).cpu()), dict(cos_sin=torch.zeros(9, 64, 2, **there)),
+               dict(cos_sin=torch.zeros(0, 32, 2, **there)), dict(cos_sin=torch.zeros(9, 32, 2, dtype=F64, **there)), dict(cos_sin=torch.zeros(9, 32, 2)),
+               dict(q_out=rows(3, 256)), dict(q_out=rows(2, 200)), dict(q_out=rows(2, 257)[:, 1:])):
+        a = {**good, "qkv": rows(2, 512), "cos_sin": None, **kw}
+        with pytest.raises((TypeError, ValueError)):
+            lowbit.rope_append8(a.pop("qkv"), a.pop("cos_sin"), **a)
+    one = (_i([0, 2], "cuda"), _i([0], "cuda"), _i([[0, 1]], "cuda"))
+    for args, total in (((one[0].cpu(), *one[1:]), 2), ((one[0].long(), *one[1:]), 2), (one, -1), (one, 1 << 31), ((one[0], one[1], one[2][0]), 2), ((one[0][:1], *one[1:]), 2)):
+        with pytest.raises((TypeError, ValueError)):
+            lowbit.read8(cache, *args, total=total)
+    base = dict(new_lens=_i([1], "cuda"), ctx_lens=_i([0], "cuda"), block_tables=_i([[0]], "cuda"), free_pages=_i([0, 1], "cuda"), ring=_i([0, 2], "cuda"),
+                block_size=16, max_tokens=4)
+    for kw in (dict(new_lens=_i([], "cuda")), dict(ctx_lens=_i([0, 1], "cuda")), dict(ctx_lens=_i([0])), dict(ring=_i([0], "cuda")), dict(free_pages=_i([], "cuda")),
+               dict(block_size=12), dict(max_tokens=-1), dict(max_tokens=1 << 31), dict(ctx_out=_i([0, 0], "cuda")), dict(ctx_out=_i([0])),
+               dict(ring_out=torch.zeros(2, **there)), dict(new_lens=torch.tensor([1], **there)), dict(block_size=1 << 30), dict(block_size=1 << 62),
+               dict(new_lens=torch.zeros(5000, dtype=I32, **there), ctx_lens=torch.zeros(5000, dtype=I32, **there), block_tables=torch.zeros(5000, 1, dtype=I32, **there))):
+        with pytest.raises((TypeError, ValueError)):
+            lowbit.page_step(**{**base, **kw})
+    codes, s = torch.zeros(16, 64, dtype=torch.uint8, **there), torch.ones(16, 1, dtype=BF16, **there)
+    w = lowbit.Weight4(codes, s)
+    for args in ((codes.int(), s), (codes, s.float()), (codes, s.cpu()), (codes, torch.ones(16, 3, dtype=BF16, **there)), (codes, s, s)):
+        with pytest.raises((TypeError, ValueError)):
+            lowbit.Weight4(*args)
+    for n in (2, 20, 70):
+        x = rows(n, 128)
+        for args in ((x.float(), w), (x.cpu(), w), (x[:, :64], w), (x, w, torch.zeros(16, **there)), (x, w, rows(15)), (x, w, rows(16).cpu()), (x, w, rows(32)[::2])):
+            with pytest.raises((TypeError, ValueError)):
+                lowbit.linear4(*args)
