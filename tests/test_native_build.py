@@ -1,5 +1,8 @@
 """The build of the native libraries (``loqa_hub_amd/_native/build.py``), without compiling."""
 import importlib.util
+import os
+import re
+import runpy
 import subprocess
 
 import pytest
@@ -33,3 +36,18 @@ def test_the_module_has_the_abi_of_torch(no_compiler, monkeypatch, abi):
     assert build.build(only=("libloqa_launch.so",))
     assert f"-D_GLIBCXX_USE_CXX11_ABI={int(abi)}" in no_compiler[-1]
     assert len(no_compiler) == 1 and build.build(only=("libloqa_launch.so",)) and len(no_compiler) == 1      # up to date
+
+
+def test_trace_run_builds_what_it_loads(monkeypatch):
+    """bin/trace_run in a checkout without built libraries: it compiles every library that the models' ops load."""
+    from loqa_hub_amd.cli import trace_run
+    from loqa_hub_amd.ops import _lib
+    asked = []
+    monkeypatch.setattr(build, "build", lambda *a, only=None, **kw: asked.append(only))
+    monkeypatch.setattr(trace_run, "main", lambda: 0)
+    with pytest.raises(SystemExit) as end:
+        runpy.run_path(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "bin", "trace_run"), run_name="__main__")
+    assert end.value.code == 0 and len(asked) == 1
+    with open(_lib.__file__) as f:
+        loaded = set(re.findall(r'"(libloqa_\w+\.so)"', f.read()))
+    assert len(loaded) == 5 and (asked[0] is None or loaded <= set(asked[0]))
