@@ -1,5 +1,6 @@
 """``ops.lowbit``: the paged 8-bit cache and what writes and reads it, pages handed out on the GPU, 4-bit products."""
 import math
+import threading
 
 import pytest
 import torch
@@ -832,6 +833,38 @@ def test_two_streams():
     torch.cuda.synchronize()
     for i in (0, 1):
         assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.gpu
+def test_calls_from_threads():
+    """Threads on streams of their own and on one stream together: each gets what it gets alone."""
+    H, G, D, P, n = 8, 2, 128, 16, 4
+    w = lowbit.Weight4(*(t.cuda() for t in lowbit.quantize4(torch.randn(320, 4096, generator=torch.Generator().manual_seed(1)), 64, True)))
+    work = []
+    for i in range(n):
+        q, c, *rest = _attend_case((1,) if i % 2 else (9,), (9000,), H, G, D, P, INT8, seed=i)
+        x = torch.randn(33 + i, 4096, device="cuda", generator=torch.Generator("cuda").manual_seed(i)).to(BF16)
+        work.append((x, q.cuda(), _to(c, "cuda"), *(t.cuda() for t in rest)))
+
+    def both(x, q, cache, cu, ctx, bt):
+        return lowbit.linear4(x, w), lowbit.attention8(q, cache, cu, ctx, bt, n_heads=H, max_q=q.shape[0])
+    want = [both(*a) for a in work]
+    torch.cuda.synchronize()
+    for streams in ([torch.cuda.Stream() for _ in range(n)], [torch.cuda.current_stream()] * n):
+        got = [None] * n
+
+        def loop(i):
+            with torch.cuda.stream(streams[i]):
+                got[i] = [both(*work[i]) for _ in range(20)]
+                streams[i].synchronize()
+        threads = [threading.Thread(target=loop, args=(i,)) for i in range(n)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        for i in range(n):
+            assert got[i] is not None and all(torch.equal(a, b) for y in got[i] for a, b in zip(y, want[i])), i
 
 
 # ------------------------------------------------------------------ refusals
