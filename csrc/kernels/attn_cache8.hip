@@ -205,9 +205,9 @@ __device__ __forceinline__ void a8_join(const Attn8Args& A, size_t unit, int n, 
 // workgroups of a sequence parts of its keys. A tile is 8 KB to the bf16 form's 16 and as much work: page numbers are scalars
 // that no wait precedes (kept in an array they went through LDS, and a tile waited for the next one's: 32 x 4000 keys x 8
 // heads of 128 66 us), values are asked of LDS ahead of the exponentials. us, cold caches, pages of 16 (bf16 form): 32 x 4000 keys x 8
-// heads of 128 49 (96), 5.1 TB/s; 1 x 100000 38, 5.4; 256 x 1000 90 (159); 8 x 600 10 (13); 1 x 600 6.9 (10.9); 64 x 300 13 (21); 8 x
+// heads of 128 50 (96), 5.0 TB/s; 1 x 100000 38, 5.4; 256 x 1000 92 (159); 8 x 600 10 (13); 1 x 600 6.8 (10.9); 64 x 300 13 (21); 8 x
 // 1500 x 20 of 64 13 (19). Two tiles of rows share what is widened: 32 rows behind 1 x 30000 keys x 8 heads of 128 37 (the prompt form below
-// 65), 16 x 4000 41 (56), 32 x 1000 21 (36). Four of them, with one workgroup a compute unit: 64 rows 62 (65), 76 (57), 33 (37); left out.
+// 65), 16 x 4000 40 (56), 32 x 1000 20 (36). Four of them, with one workgroup a compute unit: 64 rows 62 (65), 76 (57), 33 (37); left out.
 //
 //   S^T = K Q^T   : 16 x 16 x 32 MFMAs; a lane reads 16 codes of a key at once, the K slots of two MFMAs
 //   O^T += V^T P^T: eight keys of one column by a transposing read of bytes; P^T is the accumulator as it stands
@@ -501,8 +501,8 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R, RT>::FIT)) void attn8
 // What bounds it: at 128 columns two waves share a SIMD (registers, and 64 KB of stages), and of 2400 cycles that a tile of one takes
 // there its vector instructions have 1500 (310 of them, 32 exponentials among them, 40 to 90 to widen its share of the codes),
 // its 32 MFMAs 1024, LDS 1100; a third of a wave's time is waiting to issue, a quarter for LDS and at the barrier.
-// 2048 causal rows x 32 query heads over 8 of 128 columns 56 us (0.61 PFLOP/s; the bf16 form,
-// whose keys and values go to LDS as they are, 56), 1024 31, 512 17; 3 x 113 rows behind 5000 keys, 64 columns, 34.
+// 2048 causal rows x 32 query heads over 8 of 128 columns 57 us (0.61 PFLOP/s; the bf16 form,
+// whose keys and values go to LDS as they are, 56), 1024 28, 512 18; 3 x 113 rows behind 5000 keys, 64 columns, 34.
 // Taken back: pages and addresses on the scalar unit (fewer vector instructions, but a chain of scalar ones in their place: 58 -> 66 us);
 // the longest parts first, counted by a lane for each block (2048 rows 79); six and eight fragments of K in flight, halves of a chunk
 // swapped against bank conflicts of the writes (nothing); a wave's priority raised for products or for weights, the maxima in 16

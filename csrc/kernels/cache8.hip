@@ -7,12 +7,13 @@
 //
 //   s = max(f(max |new rows of the page|), s before (if the page held rows), 2^-100),   f(a) = a / 127 or 2^ceil(log2(a / 448))
 //
-// in f32 from the bf16 rows to the one rounding (products and sums unfused, so that the codes are those of the plain
-// formulas bit for bit). Where s grows, the page's older rows are rounded again to it.
+// in f32 from the bf16 rows to the one rounding (products and sums unfused and quotients rounded once, so that the codes are
+// those of the CPU form bit for bit; torch on the GPU divides by 127 as a product with its reciprocal, and its int8 scales are an ulp off
+// now and then). Where s grows, the page's older rows are rounded again to it.
 // A wave has one page of one head, keys or values, and with it all that touches that scale: no atomics, and the
 // same codes whatever else is in the batch. Bound by latency for token steps (metadata, page number, scale and rows
-// one behind the other: eight replies x 32 + 2 x 8 heads of 128 4.4 us), by the bytes of qkv and q for prompts (2048 such rows, 46 MB, 13.0 us,
-// 3.6 TB/s; with each head's load behind the store of the one before, and keys and values last, 14.4; 16 bytes a load: no faster). Rows of a page are read once and kept where a wave has no more than AP_DEEP of them a lane (331 rows x 5, pages of 32 x 64
+// one behind the other: eight replies x 32 + 2 x 8 heads of 128 4.7 us), by the bytes of qkv and q for prompts (2048 such rows, 46 MB, 11 us,
+// 4.2 TB/s, the median of 12 calls under the profiler, 13 in another run; with each head's load behind the store of the one before, and keys and values last, 14.4; 16 bytes a load: no faster). Rows of a page are read once and kept where a wave has no more than AP_DEEP of them a lane (331 rows x 5, pages of 32 x 64
 // columns 8.0 -> 6.4 us).
 struct AppendArgs {
   const bf16_t* qkv;
@@ -243,8 +244,10 @@ extern "C" int loqa_read8(const void* k, const void* v, const void* ks, const vo
 // bisection of the sums; a token's page follows from the ring itself, so nothing waits for the table. What a caller may
 // update in place (lengths, the ring's head and count) is written by the last workgroup to have read it (without a ticket there
 // is one workgroup).
-// All or nothing: with a status nothing changes. Bound by its launch and the chain metadata, sums, ring, slots: 3.9 us for eight
-// sequences, 7.3 for 500 with 32000 tokens (5 us are the sums over all sequences and their barriers).
+// All or nothing: with a status nothing changes. Bound by its launch and the chain metadata, sums, ring, slots: 4.1 us for eight
+// sequences of a token each. 500 of them take 5.7, one pass of the sums too, but nine steps of each bisection and 500 entries of every
+// output; as many with 6000 tokens 6.5, with 32000 7.2: a token's bisection, its 64-bit remainder and the page that it then asks for, and up to
+// 64 workgroups that meet at one ticket. (Eight sequences with 24000 tokens 5.4.)
 struct PageArgs {
   const int *n, *ctx;
   int* table;

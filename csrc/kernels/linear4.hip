@@ -11,7 +11,7 @@
 // and the group's scale enters in f32. Products of whole numbers up to 143 with bf16 are exact, and what f32 sums lose, 2^-24
 // of terms up to 143 |x| where the result's own are up to 15 |x|, is far below the result's rounding to bf16.
 // (With sums of x from an MFMA of ones and the subtraction in f32, vector instructions bounded small groups: 28672 x 4096 for
-// eight rows in groups of 64 with zeros 20 us, 17 now.)
+// eight rows in groups of 64 with zeros 20 us; 17 to 19 by that clock, launches in a replayed graph, 14.3 among other calls.)
 #include "common.h"
 
 #define L4_TILE 16                     // features of a tile
@@ -278,7 +278,7 @@ __device__ __forceinline__ void l4_lds4(const void* at, unsigned dst) {
 // fragment are in different banks). K is divided among `parts` workgroups; the last of them to arrive adds up what all have
 // left, in order.
 // Bound by its waves' issue, a SIMD's MFMAs (two for each step where zeros differ), and what each block waits for the one barrier: 64 rows
-// x 28672 x 4096 37 us where the bytes take 13, 32 rows 24, 64 x 4096 x 4096 10.6, 32 x 4096 x 14336 14. (Each wave reading x from L2
+// x 28672 x 4096 37 us where the bytes take 13, 32 rows 25, 64 x 4096 x 4096 10.1, 32 x 4096 x 14336 14. (Each wave reading x from L2
 // itself, K divided within a workgroup: 46, 30, 17.7, 31; x staged through registers, a block ahead: 39, 26, 13, 19; a ring of four
 // blocks leaves room for fewer workgroups: 42 for the first.)
 template <int MT, int FT, int GS, bool Z> struct L4Rows {

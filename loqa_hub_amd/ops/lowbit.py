@@ -14,7 +14,7 @@ Sequences are given as everywhere: ``cu_q`` [B + 1] int32 bounds each sequence's
 int32 its tokens with this step's, ``block_tables`` [B, max_blocks] int32 its pages; row i of a sequence
 of n rows stands at position ctx - n + i. Rows behind the last sequence are neither read nor written.
 Page numbers outside of the cache are never followed: nothing is appended there, and attention takes its
-keys as masked. A page that gets rows belongs to one sequence; full pages may be shared.
+keys as masked. Appends and token steps take up to 65535 sequences a call. A page that gets rows belongs to one sequence; full pages may be shared.
 """
 from __future__ import annotations
 
@@ -75,7 +75,8 @@ class Cache8:
     A page's scale starts anew with the row at its first place and only grows until the next such row; its
     older rows are rounded again where it grows, so a page filled row by row is off by up to a step where one filled at
     once is off by half a step. e4m3 scales are powers of two, whose growth rounds nothing again but the smallest
-    entries. Scales below 2^-100, negative ones among them, count as 2^-100 everywhere. Page sizes are
+    entries. Codes are numbers: e4m3's NaN, which no append writes, may reach every row of a feed
+    that it is cached for. Scales below 2^-100, negative ones among them, count as 2^-100 everywhere. Page sizes are
     powers of two from 16 on."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "kind", "n_blocks", "n_kv", "block_size", "head_dim", "cuda")
@@ -212,12 +213,12 @@ def attn8_plan(max_q: int, group: int, units: int, keys: int, D: int) -> tuple[i
 
 def _token_plan(form: int, rows: int, units: int, keys: int, D: int) -> tuple[int, int, int, int, int]:
     # Two workgroups for each compute unit, no part of less than a tile for each wave, and, since a unit's parts are joined by one of
-    # them, about the square root of its keys. us by parts, heads of 128 (contexts x keys x kv heads): 16 x 4000 x 8 40.7 (1), 33.6
-    # (2), 35.1 (3), 31.0 (4), 35.8 (6); 12 x 4000 x 8 38.1 (1), 26.1 (2), 30.6 (3), 26.7 (4), 29.8 (6); 24 x 4000 x 8 45.4 (1), 48.8
-    # (2), 32 of them 55.5 (1), 58.4 (2); 1 x 2000 x 8 of 8 rows 20.5 (1), 11.4 (4), 9.8 (8), 9.5 (16), of 32 rows 26.2, 17.6, 15.9,
-    # 18.6; 1 x 30000 x 8 of 8 rows 25.4 (16), 22.6 (24), 22.9 (32), 25.0 (48), of 32 rows 37.0, 35.7, 37.2, 45.3; 64 columns: 1 x
-    # 20000 x 1 of 5 rows 16.2 (16), 13.3 (24), 12.7 (32), 11.9 (48); 32 x 4000 x 8 36.7 (1), 31.2 (2), 32.1 (4). Many rows of few keys: 1
-    # x 300 x 8 of 32 rows 10.0 (1), 12.5 (3), 8 x 700 14.4 (1), 16.1 (4), 8 x 1500 21.8 (1), 19.9 (2), 20.4 (6)
+    # them, about the square root of its keys. us by parts, heads of 128 (contexts x keys x kv heads): 16 x 4000 x 8 39.4 (1), 31.7
+    # (2), 33.7 (3), 31.2 (4), 35.7 (6); 12 x 4000 x 8 37.9 (1), 26.4 (2), 30.6 (3), 26.7 (4), 30.1 (6); 24 x 4000 x 8 45.9 (1), 46.7
+    # (2), 32 of them 56.1 (1), 56.8 (2); 1 x 2000 x 8 of 8 rows 20.5 (1), 11.5 (4), 9.9 (8), 9.4 (16), of 32 rows 26.7, 17.8, 16.1,
+    # 19.2; 1 x 30000 x 8 of 8 rows 25.4 (16), 22.8 (24), 23.0 (32), 25.1 (48), of 32 rows 37.1, 35.8, 37.1, 45.2; 64 columns: 1 x
+    # 20000 x 1 of 5 rows 15.4 (16), 12.9 (24), 12.7 (32), 11.6 (48); 32 x 4000 x 8 34.8 (1), 30.4 (2), 31.1 (4). Many rows of few keys: 1
+    # x 300 x 8 of 32 rows 10.1 (1), 12.8 (3), 8 x 700 14.7 (1), 16.0 (4), 8 x 1500 22.4 (1), 20.3 (2), 20.5 (6)
     parts, few = SLOTS // units, rows * D <= 1024
     if D == 128 and parts < 3:
         parts = 1
@@ -229,9 +230,9 @@ def _token_plan(form: int, rows: int, units: int, keys: int, D: int) -> tuple[in
 def _prompt_plan(rows: int, units: int, keys: int, D: int) -> tuple[int, int, int, int, int]:
     blocks, most = -(-rows // PROMPT_ROWS), max(1, -(-keys // 64))
     # parts of four tiles at least, about the square root of the keys as above. us by parts: 1 x 30000 keys x 8 kv heads of 128 columns, 48
-    # rows 665 (1), 100 (8), 65 (16), 57 (24), 56 (32); 1 x 4000 85 (1), 25.8 (8), 25.3 (12), 26.5 (16), 36 (32); 1 x 700 21 (1), 16.0
-    # (4), 19.2 (12); 3 x 113 rows x 4 behind 5000 x 8 of 64 82 (1), 39 (4), 35 (5), 40 (6), 37 (8); 1024 x 4 causal rows x 8 of 64 22.9
-    # (1), 20.6 (2), 22.8 (3), of 128 31.3, 29.3, 31.3
+    # rows 657 (1), 97 (8), 62 (16), 53 (24), 51.3 (30 and 32); 1 x 4000 85 (1), 24.0 (8), 23.4 (12), 23.9 (16), 31 (32); 1 x 700 21 (1),
+    # 14.8 (4), 17.1 (12); 3 x 113 rows x 4 behind 5000 x 8 of 64 82 (1), 42 (4), 36 (5), 41 (6), 35 (8); 1024 x 4 causal rows x 8 of 64
+    # 21.5 (1), 19.6 (2), 22.3 (3), of 128 29.0, 28.0, 29.8
     parts = max(1, min(SLOTS // (units * blocks), most // 4, math.isqrt(keys // 32), 32))
     return (0, parts, -(-most // parts), units * blocks * parts * PROMPT_ROWS * (D + 4), units * blocks) if parts > 1 else (0, 1, most, 0, 0)
 
@@ -245,7 +246,9 @@ def attention8(q: torch.Tensor, cache: Cache8, cu_q: torch.Tensor, ctx_lens: tor
     ctx - n + i (all ctx of them where not ``causal``). ``max_q`` bounds the rows of a sequence, ``max_k``
     its context where the host knows a smaller bound than the block table's (it only chooses the split of the keys: in
     how many parts they are summed up follows from the whole call). ``scale`` is 1 / sqrt(D) by default. Rows that see no
-    key give zeros. Returns [T, H * D] bf16 (``out`` where given)."""
+    key give zeros. The longest feed chooses one form and one split for all of a call: replies of a token beside a chunk of a prompt run as
+    prompts, each walking its keys alone (us: eight replies of 4000 keys beside 512 rows 113, in two calls 38; one of 100000 keys beside
+    them 1080, in two 62), so a program that knows its lengths calls once for each. Returns [T, H * D] bf16 (``out`` where given)."""
     H, G, D = n_heads, cache.n_kv, cache.head_dim
     _need(H > 0 and H % G == 0, "n_heads must be a multiple of the cache's heads")
     _need(max_q >= 0 and (max_k is None or max_k >= 0), "max_q and max_k")
@@ -424,7 +427,8 @@ def linear4_plan(M: int, N: int, K: int) -> tuple[int, int, int, int]:
 
 def linear4(x: torch.Tensor, w: Weight4, b: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] bf16 times the transpose of a 4-bit weight (+ bias [N] bf16): [..., N] bf16, summed up in f32. Made for
-    the few rows of token steps; more than 64 read the weight again for every 64. An infinite or NaN entry of x makes its row NaN, and so may
+    the few rows of token steps; more than 64 read the weight again for every 64. Rows that do not start at 16 bytes, and x of
+    other than two dimensions, are copied first. An infinite or NaN entry of x makes its row NaN, and so may
     one past 2^112 (sums of 143 times a group's entries stay within f32 up to there)."""
     fast = None
     if w.cuda:
