@@ -404,7 +404,7 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R, RT>::FIT)) void attn8
 #pragma unroll
       for (int j = 0; j < 8; ++j) mx = fmaxf(mx, st[r][j >> 2][j & 3]);
       mx = a8_max16(fl_max32(mx));
-      if (__any(mx > m_run[r] + A8_MOST)) {      // as in the prompt form
+      if (__any(mx - m_run[r] > A8_MOST)) {      // as in the prompt form; the difference is what the weights have
         const float m_new = fmaxf(m_run[r], mx - A8_BELOW), alpha = __builtin_amdgcn_exp2f(m_run[r] - m_new);
         m_run[r] = m_new;
         l_run[r] *= alpha;
@@ -663,7 +663,7 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     float4v lv = *reinterpret_cast<const float4v*>(sc + 4), inv = *reinterpret_cast<const float4v*>(sc + 8);
     float16v s[2];
     c8_h8 kf[KR], vf[VR], p[4];
-    float sum[4], c[4], top[4];
+    float sum[4], c[4], top[4], off[4];
     auto kread = [&](int u) __attribute__((always_inline)) { kf[u % KR] = *fl_lds<c8_h8>(kb[u % NS] + (stage * L::STAGE + 32 * (u / NS) * D * 2)); };
     auto vread = [&](int v) __attribute__((always_inline)) {
       const unsigned a = vb[v % NDT] + (stage * L::STAGE + 16 * (v / NDT) * D * 2);
@@ -681,12 +681,11 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     };
     // scores j of group g (16 keys of a page): 2^(x c + log2 vs - m)
     auto weights = [&](int g, int j0, int j1) __attribute__((always_inline)) {
-      const float off = lv[g] - m;
 #pragma unroll
       for (int j = j0; j < j1; j += 2) {
         typedef float f2 __attribute__((ext_vector_type(2)));
-        const f2 e = {__builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j], c[g], off)),
-                      __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j + 1], c[g], off))};
+        const f2 e = {__builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j], c[g], off[g])),
+                      __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + j + 1], c[g], off[g]))};
         const c8_h2 w = __builtin_convertvector(e, c8_h2);
         sum[g] = j == 0 ? e[0] + e[1] : sum[g] + (e[0] + e[1]);    // in f32: a weight that f16 has as zero still counts for a page of small values
         p[g][j] = w[0];
@@ -736,14 +735,20 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) tops(g, 0, 8);
-    // x c + log2 vs with c above zero: the largest product of a group is its largest score
+    // x c + log2 vs with c above zero: the largest product of a group is its largest score. The reference stays where it is while no
+    // weight passes 2^15, up to which f16 keeps 11 bits (a prompt's first tiles nearly always raise some row of the wave): asked of the
+    // weights' own exponents, as scores past 2^23 have steps that a sum of 15 would be rounded to
     float mx = -INFINITY;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) mx = fmaxf(mx, fmaf(top[g], c[g], lv[g]));
-    // the reference stays where it is while no weight passes 2^15, up to which f16 keeps 11 bits: a prompt's first tiles nearly
-    // always raise some row of the wave
-    mx = fl_max32(mx);
-    if (__any(mx > m + A8_MOST)) {
+    for (int g = 0; g < 4; ++g) {
+      off[g] = lv[g] - m;
+      mx = fmaxf(mx, fmaf(top[g], c[g], off[g]));
+    }
+    if (__any(mx > A8_MOST)) {
+      mx = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) mx = fmaxf(mx, fmaf(top[g], c[g], lv[g]));
+      mx = fl_max32(mx);
       const float m_new = fmaxf(m, mx - A8_BELOW), alpha = __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
       l *= alpha;
@@ -751,6 +756,8 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
       for (int d = 0; d < NDT; ++d)
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[d][j] *= alpha;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) off[g] = lv[g] - m;
     }
     weights(0, 0, 8);
     weights(1, 0, 8);

@@ -518,6 +518,37 @@ def test_many_keys_behind_a_dominant_one(dtype, H, dev):
     assert ((got - o).abs() <= (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -14) * o + L * 2.0 ** -32).all(), (float(got.min()), float(got.max()), o)
 
 
+@KINDS
+@pytest.mark.parametrize("H", [4, 20, 40, 130])
+@pytest.mark.parametrize("most", [20, 23, 24.5, 25.5])
+@pytest.mark.parametrize("dev", DEVICES)
+def test_scores_as_large_as_their_steps(dtype, H, most, dev):
+    """Scores of 2^20 to 2^25 (base two) that f32 holds in steps of up to four: whatever these make of them, results stay between the
+    smallest and the largest value."""
+    D, P, L = 64, 16, 1500
+    g = torch.Generator().manual_seed(int(most * 2) + H)
+    cache = lowbit.Cache8.empty(-(-L // P), 1, P, D, dtype)
+    code = 127 if dtype is INT8 else 128
+    k = torch.zeros(cache.k.shape)
+    k[..., 0] = code
+    k[..., 1] = (torch.arange(k.shape[0]) * 127 / k.shape[0]).round()[:, None, None]        # scores that rise with the keys
+    k[..., 2] = torch.randint(-1, 2, k.shape[:3], generator=g).float()
+    cache.k.view(torch.uint8)[:] = k.to(dtype).view(torch.uint8)
+    cache.v.view(torch.uint8)[:] = (torch.randint(32, 97, k.shape, generator=g).float()).to(dtype).view(torch.uint8)
+    cache.k_scale.fill_(1.0)
+    cache.v_scale.copy_(0.6 + torch.rand(cache.v_scale.shape, generator=g))
+    q = torch.zeros(1, H * D)
+    base = 2.0 ** most / code
+    q[0, 0::D] = base * torch.where(torch.arange(H) % 5 == 4, -1.0, 1.0)
+    q[0, 1::D] = 2.0 ** (3 + 6 * torch.rand(H, generator=g)) / 127                          # by 8 to 512
+    q[0, 2::D] = 1.0
+    bt = torch.arange(cache.n_blocks, dtype=I32, device=dev)[None]
+    got = lowbit.attention8(q.to(BF16).to(dev), _to(cache, dev), _i([0, 1], dev), _i([L], dev), bt, n_heads=H, max_q=1, scale=math.log(2), max_k=1).cpu().float()
+    v = cache.v.float() * cache.v_scale[..., None, None]
+    # rounded to bf16, weights to f16 while their sum is not
+    assert got.isfinite().all() and (got <= v.max() * (1 + 2.0 ** -7)).all() and (got >= v.min() * (1 - 2.0 ** -7)).all()
+
+
 # ------------------------------------------------------------------ pages
 def _pages_case(new, ctx, P, width, free, head=0, spare=2, seed=0):
     held = [-(-c // P) for c in ctx]
