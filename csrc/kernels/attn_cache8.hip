@@ -501,7 +501,7 @@ __global__ __launch_bounds__(A8_WAVES * 64, (A8Token<D, R, RT>::FIT)) void attn8
 // What bounds it: at 128 columns two waves share a SIMD (registers, and 64 KB of stages), and of 2400 cycles that a tile of one takes
 // there its vector instructions have 1500 (310 of them, 32 exponentials among them, 40 to 90 to widen its share of the codes),
 // its 32 MFMAs 1024, LDS 1100; a third of a wave's time is waiting to issue, a quarter for LDS and at the barrier.
-// 2048 causal rows x 32 query heads over 8 of 128 columns 57 us (0.61 PFLOP/s; the bf16 form,
+// 2048 causal rows x 32 query heads over 8 of 128 columns 58 us (0.59 PFLOP/s; the bf16 form,
 // whose keys and values go to LDS as they are, 56), 1024 28, 512 18; 3 x 113 rows behind 5000 keys, 64 columns, 34.
 // Taken back: pages and addresses on the scalar unit (fewer vector instructions, but a chain of scalar ones in their place: 58 -> 66 us);
 // the longest parts first, counted by a lane for each block (2048 rows 79); six and eight fragments of K in flight, halves of a chunk
@@ -650,7 +650,7 @@ __global__ __launch_bounds__(256, 2) void attn8_prompt_kernel(Attn8Args A) {
   // A tile: the scores of its first 32 keys, beside which the next tile is widened; those of the second 32; the maxima, which move the
   // reference where they have to, and the weights of the first keys; the values' products of these beside the weights of the second;
   // those of the second beside the addresses of the tile after the next. (One after the other, stages toggled in registers: the 2048
-  // rows above 58 us, 56 now; the first weights beside the second scores, and once more where the reference moves: no faster.)
+  // rows above 58 us, 56 so; the first weights beside the second scores, and once more where the reference moves: no faster.)
   constexpr int KR = 4, VR = 4;                              // fragments in flight + 1
   // rows of this wave that some key of a tile from here on is hidden from, or that end in it
   const int edge = min(f.keys, A.causal ? f.past + (r0 + wave * 32) / Gq + 1 : f.keys) - A8P_KEYS;
